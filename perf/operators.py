@@ -134,7 +134,8 @@ def _pack(code, d, m, value_plane):
     groups, size = (8, 2) if value_plane else (4, 4)
     by = by.unflatten(-1, (groups, size)).transpose(-2, -3).reshape(s, -1)
     par = torch.stack([d, m], -1).transpose(1, 2).reshape(s, -1).view(torch.uint8)
-    return torch.cat([by, par], 1).contiguous()
+    whole = torch.cat([by, par], 1)
+    return torch.nn.functional.pad(whole, (0, -whole.shape[1] % 16)).contiguous()           # a sequence begins at 16 bytes
 
 
 def _unpack(buf, rows, kv_heads, dim, value_plane):
@@ -144,7 +145,7 @@ def _unpack(buf, rows, kv_heads, dim, value_plane):
     groups, size = (8, 2) if value_plane else (4, 4)
     by = buf[:, :cut].reshape(s, kv_heads, rows, groups, nb, size).transpose(-2, -3).reshape(s, kv_heads, rows, nb, 16)
     code = torch.stack([by & 15, by >> 4], -1).flatten(-2).transpose(1, 2)
-    par = buf[:, cut:].contiguous().view(torch.float16).reshape(s, kv_heads, rows, nb, 2).transpose(1, 2)
+    par = buf[:, cut:cut + kv_heads * rows * dim // 8].contiguous().view(torch.float16).reshape(s, kv_heads, rows, nb, 2).transpose(1, 2)
     return code, par[..., 0], par[..., 1]
 
 
@@ -155,7 +156,7 @@ def prepare(case, seed):
     if c["op"] == "store":
         st["new_k"], st["new_v"] = _rows(gen, (S, c["tokens"], H), D), _rows(gen, (S, c["tokens"], H), D)
         if c["bits"] == 4:
-            st["k"] = torch.zeros(S, H * cap * (D // 2 + D // 8), dtype=torch.uint8, device="cuda")
+            st["k"] = torch.zeros(S, -(-H * cap * (D // 2 + D // 8) // 16) * 16, dtype=torch.uint8, device="cuda")
         else:
             st["k"] = torch.zeros(S, cap, H, D, dtype=torch.float16, device="cuda")
         st["v"] = torch.zeros_like(st["k"])
@@ -415,7 +416,7 @@ def _exact_rows(st, which):
     byte = ((i // 8) * nb + b) * 4 + (i % 8) // 2 if which == "k" else ((i // 4) * nb + b) * 2 + (i % 4) // 2
     rows = st[which][:, :H * cap * D // 2].reshape(S, H, cap, D // 2)[..., byte].int()
     code = (rows >> (4 * (i % 2))) & 15
-    par = st[which][:, H * cap * D // 2:].contiguous().view(torch.float16).reshape(S, H, cap, nb, 2).double()
+    par = st[which][:, H * cap * D // 2:H * cap * (D // 2 + D // 8)].contiguous().view(torch.float16).reshape(S, H, cap, nb, 2).double()
     return (par[..., 0][..., b] * code + par[..., 1][..., b]).transpose(1, 2)
 
 
