@@ -271,6 +271,88 @@ int kcb_set_rows_f16(const float* src_dev, const int64_t* idx_dev, void* dst_dev
 int kcb_flash_attn_f16(const float* q_dev, const void* k_dev, const void* v_dev, const void* mask_dev, float* out_dev,
                        const int* fa_dims15, float scale, void* stream);
 
+/* ---- KV cache for long contexts: fp16 or 4 bits, masked and biased attention, eviction ----------------------------------
+ * No counterpart in the reference, whose cache is fp32 or fp16 and whose attention has neither caps, biases nor
+ * documents.  A cache is a description of device buffers that the caller owns; the calls below only enqueue work on
+ * `stream` and update the buffers in stream order, so a decode step of them can be captured once and replayed while the
+ * counts grow on the device.
+ *
+ * bits = 16: k and v are fp16 rows of head_dim, at (seq, slot, head) = base + seq * k_seq + slot * k_row + head * k_head
+ *            halves (the decoder's [capacity][kv_heads][head_dim] is k_row = kv_heads * head_dim, k_head = head_dim);
+ *            strides are multiples of 8, bases 16-byte aligned.  Values are converted as kcb_set_rows_f16 converts.
+ * bits = 4:  k and v are buffers of kcb_cache_bytes each, 16-byte aligned; the strides are not read.  A block of 32
+ *            channels of a row has a minimum m = fp16(min) and a scale d = fp16((max - min) * (1 / 15)) by fp32
+ *            steps, and every channel a code in 0..15, (x - m) / d rounded to the nearest integer: value d * code + m,
+ *            0.625 bytes each.
+ *            Inputs are clamped to fp16's range, NaN counts as 0.  Per sequence (16-byte multiple): nibbles
+ *            [kv_heads][capacity][head_dim / 2], then {d, m} as fp16 [kv_heads][capacity][head_dim / 32][2].  A key row
+ *            holds for c = 0..3 the 4 bytes of channels 8c..8c+7 of every block, a value row for g = 0..7 the 2 bytes
+ *            of channels 4g..4g+3 of every block; two channels to a byte, the lower one in the low nibble.
+ * n_keys[seq]: rows in use (slots 0 .. n_keys - 1; what lies behind is never read); NULL: all `capacity` rows.
+ * next_pos[seq]: tokens seen so far, the position of the next one; NULL: n_keys (nothing was evicted).
+ * positions[seq][head][slot]: the position of the row in a slot; NULL: slot = position.
+ * weights[seq][head][slot]: attention weight the row has received so far. */
+enum { KCB_CACHE_Q4 = 4, KCB_CACHE_F16 = 16 };
+typedef struct {
+    int bits, n_seqs, kv_heads, head_dim, capacity; /* head_dim: a multiple of 32, at most 256 */
+    void* k;
+    void* v;
+    int64_t k_row, k_head, k_seq, v_row, v_head, v_seq;
+    int32_t* n_keys;
+    int32_t* next_pos;
+    int32_t* positions;
+    float* weights;
+} kcb_kv_cache;
+/* Bytes of the key (or value) buffer of a cache; 0 for a shape there is none of.  Host arithmetic. */
+size_t kcb_cache_bytes(int bits, int n_seqs, int kv_heads, int head_dim, int capacity);
+/* n_tokens new rows per sequence behind the n_keys in use: fp32 [kv_heads][head_dim] at k + seq * seq_stride + token *
+ * token_stride floats (multiples of 4; k and v 16-byte aligned).  Then n_keys and next_pos grow by n_tokens; the rows'
+ * positions are next_pos + token, their weights 0.  Rows beyond the capacity are dropped and n_keys stops there. */
+int kcb_cache_append(const kcb_kv_cache* cache, const float* k_dev, const float* v_dev, int n_tokens, int64_t token_stride, int64_t seq_stride,
+                  void* stream);
+/* Slots first .. first + count - 1 of every sequence as fp32 [n_seqs][count][kv_heads][head_dim], the values that the
+ * cache stands for; zeros for slots that are not in use. */
+int kcb_cache_read(const kcb_kv_cache* cache, int first, int count, float* k_out_dev, float* v_out_dev, void* stream);
+
+/* Attention of n_tokens query tokens per sequence over the cache.  Scores are scale * q.k; softcap > 0 bends them to
+ * softcap * tanh(score / softcap); max_bias > 0 gives every head the slope 2^-(max_bias (h + 1) / H) (H: the largest power
+ * of two of heads; the heads behind it 2^-(max_bias (2 (h - H) + 1) / 2H)) and subtracts slope * |query position - key
+ * position|, or, with an additive mask, adds slope * mask instead of the mask (ggml's convention).
+ * A query sees a slot that is in use and that nothing hides:
+ *   causal != 0    the key's position is at most the query's, or below prefix[seq] (prefix may be NULL)
+ *   q_doc, k_doc   the document of the query [n_seqs][n_tokens] equals that of the slot [n_seqs][capacity]
+ *   mask           fp16, mask[seq * mask_seq + token * mask_token + slot], added to the score; -inf hides
+ * Query positions are q_pos[n_seqs][n_tokens], or by default those of the newest n_tokens tokens (next_pos - n_tokens +
+ * token); a query in front of its sequence sees nothing.  A row that sees nothing gives zeros.
+ * Documents and masks go by slot, so a cache with positions refuses them (InvalidValue).
+ * accumulate != 0 also adds every key's softmax weights, summed over the query rows of its kv head, to cache->weights.
+ * q, out: fp32 rows of head_dim at token * q_token + head * q_head + seq * q_seq floats (multiples of 4, 16-byte aligned);
+ * out must not overlap q.  head_dim 32, 64, 96, 128 or 256, else UnsupportedOperation.
+ * `workspace` (16-byte aligned, kcb_cache_attention_workspace_bytes of the same arguments, possibly 0) is used in stream order:
+ * calls that share one must not overlap. */
+typedef struct {
+    int n_tokens, heads;
+    float scale, softcap, max_bias;
+    int causal, accumulate;
+    const int32_t* prefix;
+    const int32_t* q_pos;
+    const int32_t* q_doc;
+    const int32_t* k_doc;
+    const void* mask;
+    int64_t mask_token, mask_seq;
+    int64_t q_token, q_head, q_seq, out_token, out_head, out_seq;
+} kcb_cache_attn;
+size_t kcb_cache_attention_workspace_bytes(const kcb_kv_cache* cache, const kcb_cache_attn* attn);
+int kcb_cache_attention(const kcb_kv_cache* cache, const kcb_cache_attn* attn, const float* q_dev, float* out_dev, void* workspace_dev,
+                     size_t workspace_bytes, void* stream);
+
+/* Drops rows of every sequence that holds more than `keep`: per kv head the rows whose position is next_pos - recent or later
+ * stay, then those of the greatest weight, at equal weight the lowest slot (a NaN weight goes first).  Kept rows behind
+ * slot `keep` move, with their positions and weights, into the free slots below it, the j-th into the j-th; n_keys becomes
+ * keep.  Needs n_keys, next_pos, positions and weights; 0 < keep, 0 <= recent <= keep. */
+size_t kcb_cache_evict_workspace_bytes(const kcb_kv_cache* cache, int keep);
+int kcb_cache_evict(const kcb_kv_cache* cache, int keep, int recent, void* workspace_dev, size_t workspace_bytes, void* stream);
+
 /* ---- decoder model and decode loop ----------------------------------------------------------------------
  * C view of llm::Model / llm::decodeToken / llm::makeKcBackend (llm/llm_model.hpp:100-207 of the reference;
  * model assembly as llm/gguf_model.cpp:51-106).  Weights are given as canonical GGUF blocks in HOST

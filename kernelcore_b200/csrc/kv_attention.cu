@@ -1,0 +1,36 @@
+// Attention kernels over a KV cache (kv_attention.cuh holds the mathematics and the measurements).  The Makefile compiles this
+// file once per cache format and head dimension, with KV_BITS and KV_DIM set, and once without them for the choice among them.
+#ifdef KV_BITS
+
+#include "kv_attention.cuh"
+
+namespace kcb {
+template <>
+int attn_launch<KV_BITS, KV_DIM>(const AttnP& P, bool general, bool tile, cudaStream_t st) {
+    return attn_launch_kernels<KV_DIM, KV_BITS>(P, general, tile, st);
+}
+}  // namespace kcb
+
+#else
+
+#include "common.cuh"
+#include "kv_cache.h"
+
+namespace kcb {
+template <int BITS>
+static int attn_launch_dim(const AttnP& P, int head_dim, bool general, bool tile, cudaStream_t st) {
+    switch (head_dim) {
+    case 32: return attn_launch<BITS, 32>(P, general, tile, st);
+    case 64: return attn_launch<BITS, 64>(P, general, tile, st);
+    case 96: return attn_launch<BITS, 96>(P, general, tile, st);
+    case 128: return attn_launch<BITS, 128>(P, general, tile, st);
+    case 256: return attn_launch<BITS, 256>(P, general, tile, st);
+    }
+    return KCB_UNSUPPORTED_OPERATION;
+}
+int attn_launch_bits(const AttnP& P, int bits, int head_dim, bool general, bool tile, cudaStream_t st) {
+    return bits == KCB_CACHE_F16 ? attn_launch_dim<16>(P, head_dim, general, tile, st) : attn_launch_dim<4>(P, head_dim, general, tile, st);
+}
+}  // namespace kcb
+
+#endif
