@@ -25,6 +25,7 @@ namespace kcb {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kPShift = 12.0f;  // probabilities enter the products times 2^12
+constexpr int kRowsMax = 16;      // a rows launch takes at most this many query rows per kv head; more go to a tile launch
 
 // Everything a launch needs, by value.  Strides are in elements (halves, floats).
 struct AttnP {
@@ -53,8 +54,26 @@ struct AttnP {
     int nsplit, row_tiles;
     float* part_o;   // [seq][kv head][split][row][D]
     float2* part_ml; // [seq][kv head][split][row] {maximum, sum}
-    float2* final_ml;  // [seq][kv head][row], null unless weights are accumulated
+    float2* final_ml;  // [seq][kv head][row], for the weights of a tile launch, else null
+    float* scores;     // [seq][kv head][row][capacity], for the weights of a rows launch, else null (part_ml is written then)
 };
+
+// A kernel launched with launch_dependent may start while its predecessor in the stream still runs; it touches nothing that the
+// predecessor writes before this wait.  The predecessor lets it start early with the second call.
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_dependents_may_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+template <class... P, class... A>
+inline int launch_dependent(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid, cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr, cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess) return KCB_SUCCESS;
+    cudaGetLastError();
+    return KCB_LAUNCH_FAILURE;
+}
 
 // ---- small device helpers ------------------------------------------------------------------------------------------
 __device__ __forceinline__ float ex2(float x) {
@@ -350,6 +369,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps) attn_rows_kernel(const __grid
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
     const int split = blockIdx.x, kvh = blockIdx.y / P.row_tiles, row0 = (blockIdx.y % P.row_tiles) * 8, s = blockIdx.z;
     const int n = seq_keys(P, s);
+    grid_dependents_may_launch();
     const int row = row0 + g;
     const bool valid = row < P.rows;
     const int token = (valid ? row : 0) / P.group, head = kvh * P.group + (valid ? row : 0) % P.group;
@@ -474,6 +494,12 @@ __global__ void __launch_bounds__(32 * kRowsWarps) attn_rows_kernel(const __grid
                 y[j] = t < min(limit, end) ? y[j] * ysc : -INFINITY;
             }
             mx = fmaxf(mx, y[j]);
+        }
+        if (P.scores && valid) {
+            float* sp = P.scores + ((static_cast<size_t>(s) * P.kv_heads + kvh) * P.rows + row) * P.cap + t0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (t0 + slot_of<FMT>(c, j) < end) sp[slot_of<FMT>(c, j)] = y[j];
         }
         unsigned vp[4][FMT == 16 ? 1 : NB];
         if (FMT != 16) {
@@ -624,26 +650,61 @@ __global__ void __launch_bounds__(32 * kRowsWarps) attn_rows_kernel(const __grid
         }
         if (P.nsplit > 1) {
             *reinterpret_cast<float4*>(P.part_o + (part + r) * D + ch) = a;
-            if (ch == 0) P.part_ml[part + r] = make_float2(M, L);
         } else {
             const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;
             const int tok = (row0 + r) / P.group, hd = kvh * P.group + (row0 + r) % P.group;
             *reinterpret_cast<float4*>(P.out + static_cast<size_t>(s) * P.o_seq + static_cast<size_t>(tok) * P.o_token + static_cast<size_t>(hd) * P.o_head + ch) =
                 make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
-            if (P.final_ml && ch == 0) P.final_ml[(static_cast<size_t>(s) * P.kv_heads + kvh) * P.rows + row0 + r] = make_float2(M, L);
         }
+        if (ch == 0 && (P.nsplit > 1 || P.scores)) P.part_ml[part + r] = make_float2(M, L);
     }
 }
 
 // ---- joining the splits of a row -------------------------------------------------------------------------------------------
 // One CTA per row: its warps take the splits in turn, then the warps' sums are joined through shared memory.
+// After a rows launch that also wants weights, further CTAs (blockIdx.x from `joins` on) turn 512 slots' scores into weights each:
+// weights[t] += sum over the rows of 2^(score - M) / L, the rows in order, no atomics.
+constexpr int kWeightSlots = 512;
 template <int D>
-__global__ void __launch_bounds__(128) attn_merge_kernel(const __grid_constant__ AttnP P) {
+__global__ void __launch_bounds__(128) attn_merge_kernel(const __grid_constant__ AttnP P, int joins) {
     constexpr int W = 4, Q = (D / 4 + 31) / 32;
     __shared__ float4 acc[W][D / 4];
-    __shared__ float2 ml[W];
+    __shared__ float2 ml[kRowsMax];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int row = blockIdx.x, kvh = blockIdx.y, s = blockIdx.z;
+    grid_dependency_wait();
+    if (row >= joins) {
+        const int n = seq_keys(P, s), t0 = (row - joins) * kWeightSlots;
+        if (t0 >= n) return;
+        const size_t sh = static_cast<size_t>(s) * P.kv_heads + kvh;
+        for (int r = warp; r < P.rows; r += W) {
+            float M = -INFINITY, L = 0.0f;
+            for (int i = lane; i < P.nsplit; i += 32) {
+                const float2 t = P.part_ml[(sh * P.nsplit + i) * P.rows + r];
+                if (t.y == 0.0f) continue;
+                const float m = fmaxf(M, t.x);
+                L = L * ex2(M - m) + t.y * ex2(t.x - m), M = m;
+            }
+            const float m = warp_max(M);
+            L = warp_sum(M == -INFINITY ? L : L * ex2(M - m));
+            if (lane == 0) ml[r] = make_float2(m - kPShift, L != 0.0f ? 1.0f / L : 0.0f);
+        }
+        __syncthreads();
+        float* w = P.weights + sh * P.cap;
+        const float* sc = P.scores + sh * P.rows * P.cap;
+#pragma unroll
+        for (int i = 0; i < kWeightSlots / 128; ++i) {
+            const int t = t0 + i * 128 + threadIdx.x;
+            if (t >= n) continue;
+            float sum = 0.0f;
+            for (int r = 0; r < P.rows; ++r) {
+                const float y = sc[static_cast<size_t>(r) * P.cap + t];
+                if (y != -INFINITY) sum = fmaf(ex2(y - ml[r].x), ml[r].y, sum);
+            }
+            w[t] += sum;
+        }
+        return;
+    }
     const size_t base = (static_cast<size_t>(s) * P.kv_heads + kvh) * P.nsplit;
     float M = -INFINITY;
     for (int i = threadIdx.x & 31; i < P.nsplit; i += 32) {
@@ -1143,6 +1204,7 @@ __global__ void __launch_bounds__(128) attn_weights_kernel(const __grid_constant
     extern __shared__ __align__(16) uint8_t sm[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
     const int t0 = blockIdx.x * 64, kvh = blockIdx.y, s = blockIdx.z;
+    grid_dependency_wait();
     const int n = seq_keys(P, s);
     if (t0 >= n) return;
     const uint8_t* kt = sm + C::kOffK;
@@ -1223,15 +1285,15 @@ int attn_launch_kernels(const AttnP& P, bool general, bool tile, cudaStream_t st
         }
     }
     if (int e = launch_status(); e != KCB_SUCCESS) return e;
-    if (P.nsplit > 1) {
-        attn_merge_kernel<D><<<dim3(P.rows, P.kv_heads, P.n_seqs), 128, 0, st>>>(P);
-        if (int e = launch_status(); e != KCB_SUCCESS) return e;
+    const int joins = P.nsplit > 1 ? P.rows : 0, weights = P.scores ? (P.cap + kWeightSlots - 1) / kWeightSlots : 0;
+    if (joins + weights) {
+        const int e = launch_dependent(attn_merge_kernel<D>, dim3(joins + weights, P.kv_heads, P.n_seqs), 128, 0, st, P, joins);
+        if (e != KCB_SUCCESS) return e;
     }
     if (P.final_ml) {
         static PerDeviceFlag raised;
         if (!raise_dynamic_smem(attn_weights_kernel<D, FMT>, WeightsCfg<D, FMT>::kSmem, raised)) return KCB_LAUNCH_FAILURE;
-        attn_weights_kernel<D, FMT><<<dim3((P.cap + 63) / 64, P.kv_heads, P.n_seqs), 128, WeightsCfg<D, FMT>::kSmem, st>>>(P);
-        return launch_status();
+        return launch_dependent(attn_weights_kernel<D, FMT>, dim3((P.cap + 63) / 64, P.kv_heads, P.n_seqs), 128, WeightsCfg<D, FMT>::kSmem, st, P);
     }
     return KCB_SUCCESS;
 }

@@ -28,76 +28,98 @@ __device__ __forceinline__ unsigned code_of(float x, float m, float d, float inv
     if (fabsf(fabsf(t - r) - 0.5f) < 1e-4f) r = static_cast<float>(rint((static_cast<double>(x) - static_cast<double>(m)) / static_cast<double>(d)));
     return static_cast<unsigned>(static_cast<int>(fminf(fmaxf(r, 0.0f), 15.0f)));
 }
+// Where a row's four channels 4 jr .. 4 jr + 3 stand in the 4-bit planes: the two bytes of codes, the block's parameters.
+struct Q4Place {
+    size_t codes, params;
+};
+__device__ __forceinline__ Q4Place q4_place(const kcb_kv_cache& c, size_t par_off, bool val, int h, long long t, int jr) {
+    const int nb = c.head_dim / 32, b = jr >> 3, jj = jr & 7;
+    const size_t row = static_cast<size_t>(h) * c.capacity + t;
+    const int at = val ? (jj * nb + b) * 2 : ((jj >> 1) * nb + b) * 4 + (jj & 1) * 2;
+    return {row * (c.head_dim / 2) + at, par_off + (row * nb + b) * 4};
+}
 struct AppendP {
     kcb_kv_cache c;
     const float* k;
     const float* v;
     long long tok, seq, seq_bytes, par_off;
-    int n_tokens;
+    int n_tokens, count;  // count: this launch also moves the counts on (one CTA per sequence)
 };
 __device__ __forceinline__ float cache_value(float x) {  // what a cache can hold: NaN -> 0, the rest within fp16's range
     return x != x ? 0.0f : fminf(fmaxf(x, -65504.0f), 65504.0f);
 }
+// D / 4 neighbouring threads to a row, kRowIter rows per thread and step so that as many loads are in flight.
+constexpr int kRowThreads = 256, kRowIter = 4;
+__device__ __forceinline__ void move_counts(int* n_keys, int* next_pos, int s, int capacity, int n_tokens) {
+    const long long n = static_cast<long long>(max(0, n_keys[s])) + n_tokens;
+    n_keys[s] = static_cast<int>(n < capacity ? n : capacity);
+    if (next_pos) next_pos[s] += n_tokens;
+}
 template <int BITS>
-__global__ void __launch_bounds__(256) kv_append_rows_kernel(const __grid_constant__ AppendP A) {
+__global__ void __launch_bounds__(kRowThreads) kv_append_rows_kernel(const __grid_constant__ AppendP A) {
     const kcb_kv_cache& c = A.c;
-    const int per_row = c.head_dim / 4;  // lanes of four channels
-    const long long total = static_cast<long long>(A.n_tokens) * c.kv_heads * per_row * 2;
-    const int s = blockIdx.y;
+    const int per_row = c.head_dim / 4, per_cta = kRowThreads / per_row;  // (D = 96 leaves 16 threads idle)
+    const int s = blockIdx.y, jr = threadIdx.x % per_row, r0 = threadIdx.x / per_row;
+    const unsigned rows = static_cast<unsigned>(A.n_tokens) * c.kv_heads;  // keys, then the same number of values
     const int n0 = max(0, c.n_keys[s]);
     const int first_pos = c.next_pos ? c.next_pos[s] : n0;
-    for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += static_cast<long long>(gridDim.x) * blockDim.x) {
-        const int j = static_cast<int>(i % per_row);
-        long long x = i / per_row;
-        const int h = static_cast<int>(x % c.kv_heads);
-        x /= c.kv_heads;
-        const bool val = x >= A.n_tokens;
-        const int tok = static_cast<int>(val ? x - A.n_tokens : x);
-        const long long t = static_cast<long long>(n0) + tok;
-        const float* src = (val ? A.v : A.k) + s * A.seq + tok * A.tok + static_cast<long long>(h) * c.head_dim + 4 * j;
-        const float4 f = *reinterpret_cast<const float4*>(src);
-        const bool fits = t < c.capacity;  // rows beyond the capacity are dropped
-        if (BITS == 16) {
-            if (fits) {
-                __half* dst = static_cast<__half*>(val ? c.v : c.k) + (val ? c.v_seq : c.k_seq) * s + (val ? c.v_head : c.k_head) * h + (val ? c.v_row : c.k_row) * t + 4 * j;
-                *reinterpret_cast<uint2*>(dst) = make_uint2(f32_to_f16_bits(f.x) | (f32_to_f16_bits(f.y) << 16), f32_to_f16_bits(f.z) | (f32_to_f16_bits(f.w) << 16));
+    const bool live = r0 < per_cta;
+    for (unsigned base = blockIdx.x * (per_cta * kRowIter); base < 2 * rows; base += gridDim.x * (per_cta * kRowIter)) {
+        float4 f[kRowIter];
+        unsigned hh[kRowIter], tt[kRowIter];
+#pragma unroll
+        for (int i = 0; i < kRowIter; ++i) {
+            const unsigned r = base + i * per_cta + r0, x = r < rows ? r : r - rows;
+            tt[i] = x / c.kv_heads, hh[i] = x % c.kv_heads;
+            f[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (live && r < 2 * rows) f[i] = *reinterpret_cast<const float4*>((r < rows ? A.k : A.v) + s * A.seq + tt[i] * A.tok + static_cast<long long>(hh[i]) * c.head_dim + 4 * jr);
+        }
+#pragma unroll
+        for (int i = 0; i < kRowIter; ++i) {
+            const unsigned r = base + i * per_cta + r0;
+            const bool val = r >= rows;
+            const long long t = static_cast<long long>(n0) + tt[i];
+            const int h = static_cast<int>(hh[i]);
+            const bool put = live && r < 2 * rows && t < c.capacity;  // rows beyond the capacity are dropped
+            if (BITS == 16) {
+                if (put) {
+                    __half* dst = static_cast<__half*>(val ? c.v : c.k) + (val ? c.v_seq : c.k_seq) * s + (val ? c.v_head : c.k_head) * h + (val ? c.v_row : c.k_row) * t + 4 * jr;
+                    *reinterpret_cast<uint2*>(dst) = make_uint2(f32_to_f16_bits(f[i].x) | (f32_to_f16_bits(f[i].y) << 16), f32_to_f16_bits(f[i].z) | (f32_to_f16_bits(f[i].w) << 16));
+                }
+            } else {
+                const float e[4] = {cache_value(f[i].x), cache_value(f[i].y), cache_value(f[i].z), cache_value(f[i].w)};
+                float lo = fminf(fminf(e[0], e[1]), fminf(e[2], e[3])), hi = fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3]));
+#pragma unroll
+                for (int o = 1; o < 8; o <<= 1) lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o)), hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+                const __half mh = __float2half_rn(lo), dh = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
+                const float m = __half2float(mh), d = __half2float(dh), inv = d > 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
+                unsigned w = 0;
+                if (d > 0.0f)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) w |= code_of(e[k], m, d, inv) << (4 * k);
+                if (put) {
+                    uint8_t* plane = static_cast<uint8_t*>(val ? c.v : c.k) + A.seq_bytes * s;
+                    const Q4Place at = q4_place(c, A.par_off, val, h, t, jr);
+                    *reinterpret_cast<unsigned short*>(plane + at.codes) = static_cast<unsigned short>(w);
+                    if ((jr & 7) == 0) *reinterpret_cast<__half2*>(plane + at.params) = __halves2half2(dh, mh);
+                }
             }
-        } else {
-            const float e[4] = {cache_value(f.x), cache_value(f.y), cache_value(f.z), cache_value(f.w)};
-            float lo = fminf(fminf(e[0], e[1]), fminf(e[2], e[3])), hi = fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3]));
-            const unsigned who = 0xFFu << (threadIdx.x & 24);  // the block's eight lanes come and go together (total is a multiple of 8)
-#pragma unroll
-            for (int o = 1; o < 8; o <<= 1) lo = fminf(lo, __shfl_xor_sync(who, lo, o)), hi = fmaxf(hi, __shfl_xor_sync(who, hi, o));
-            const __half mh = __float2half_rn(lo), dh = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
-            const float m = __half2float(mh), d = __half2float(dh), inv = d > 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
-            unsigned w = 0;
-            if (d > 0.0f)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) w |= code_of(e[k], m, d, inv) << (4 * k);
-            if (fits) {
-                const int nb = c.head_dim / 32, b = j >> 3, jj = j & 7;
-                uint8_t* base = static_cast<uint8_t*>(val ? c.v : c.k) + A.seq_bytes * s;
-                const long long row = static_cast<long long>(h) * c.capacity + t;
-                const int at = val ? (jj * nb + b) * 2 : ((jj >> 1) * nb + b) * 4 + (jj & 1) * 2;
-                *reinterpret_cast<unsigned short*>(base + row * (c.head_dim / 2) + at) = static_cast<unsigned short>(w);
-                if (jj == 0) *reinterpret_cast<__half2*>(base + A.par_off + (row * nb + b) * 4) = __halves2half2(dh, mh);
+            if (jr == 0 && !val && put) {
+                const size_t at = (static_cast<size_t>(s) * c.kv_heads + h) * c.capacity + t;
+                if (c.positions) c.positions[at] = first_pos + static_cast<int>(tt[i]);
+                if (c.weights) c.weights[at] = 0.0f;
             }
         }
-        if (j == 0 && !val && fits) {
-            const long long at = (static_cast<long long>(s) * c.kv_heads + h) * c.capacity + t;
-            if (c.positions) c.positions[at] = first_pos + tok;
-            if (c.weights) c.weights[at] = 0.0f;
-        }
+    }
+    if (A.count) {
+        __syncthreads();
+        if (threadIdx.x == 0) move_counts(c.n_keys, c.next_pos, s, c.capacity, A.n_tokens);
     }
 }
-// The counts move on in a launch of their own: every CTA of the rows' launch reads them.
+// Where several CTAs write a sequence's rows, each of them reads the counts: those move on in a launch of their own.
 __global__ void kv_count_kernel(int* n_keys, int* next_pos, int n_seqs, int capacity, int n_tokens) {
-    for (int s = blockIdx.x * blockDim.x + threadIdx.x; s < n_seqs; s += gridDim.x * blockDim.x) {
-        const long long n = static_cast<long long>(max(0, n_keys[s])) + n_tokens;
-        const long long p = static_cast<long long>(next_pos ? next_pos[s] : 0) + n_tokens;
-        n_keys[s] = static_cast<int>(n < capacity ? n : capacity);
-        if (next_pos) next_pos[s] = static_cast<int>(p);
-    }
+    grid_dependency_wait();
+    for (int s = blockIdx.x * blockDim.x + threadIdx.x; s < n_seqs; s += gridDim.x * blockDim.x) move_counts(n_keys, next_pos, s, capacity, n_tokens);
 }
 
 // ---- rows out ----------------------------------------------------------------------------------------------------------------
@@ -109,39 +131,46 @@ struct ReadP {
     int first, count;
 };
 template <int BITS>
-__global__ void __launch_bounds__(256) kv_read_rows_kernel(const __grid_constant__ ReadP R) {
+__global__ void __launch_bounds__(kRowThreads) kv_read_rows_kernel(const __grid_constant__ ReadP R) {
     const kcb_kv_cache& c = R.c;
-    const int per_row = c.head_dim / 4;
-    const long long total = static_cast<long long>(R.count) * c.kv_heads * per_row * 2;
-    const int s = blockIdx.y;
+    const int per_row = c.head_dim / 4, per_cta = kRowThreads / per_row;
+    const int s = blockIdx.y, jr = threadIdx.x % per_row, r0 = threadIdx.x / per_row;
+    const unsigned rows = static_cast<unsigned>(R.count) * c.kv_heads;
     const int n = c.n_keys ? min(max(0, c.n_keys[s]), c.capacity) : c.capacity;
-    for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += static_cast<long long>(gridDim.x) * blockDim.x) {
-        const int j = static_cast<int>(i % per_row);
-        long long x = i / per_row;
-        const int h = static_cast<int>(x % c.kv_heads);
-        x /= c.kv_heads;
-        const bool val = x >= R.count;
-        const int r = static_cast<int>(val ? x - R.count : x);
-        const long long t = static_cast<long long>(R.first) + r;
-        float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (t < n) {
+    if (r0 >= per_cta) return;
+    for (unsigned base = blockIdx.x * (per_cta * kRowIter); base < 2 * rows; base += gridDim.x * (per_cta * kRowIter)) {
+        uint2 w[kRowIter];  // fp16: four values; 4 bits: codes, {d, m}
+#pragma unroll
+        for (int i = 0; i < kRowIter; ++i) {
+            const unsigned r = base + i * per_cta + r0, x = r < rows ? r : r - rows;
+            const bool val = r >= rows;
+            const long long t = static_cast<long long>(R.first) + x / c.kv_heads;
+            const int h = static_cast<int>(x % c.kv_heads);
+            w[i] = make_uint2(0u, 0u);
+            if (r >= 2 * rows || t >= n) continue;
             if (BITS == 16) {
-                const __half* src = static_cast<const __half*>(val ? c.v : c.k) + (val ? c.v_seq : c.k_seq) * s + (val ? c.v_head : c.k_head) * h + (val ? c.v_row : c.k_row) * t + 4 * j;
-                const uint2 w = *reinterpret_cast<const uint2*>(src);
-                f = make_float4(half_bits_to_float(w.x & 0xFFFFu), half_bits_to_float(w.x >> 16), half_bits_to_float(w.y & 0xFFFFu), half_bits_to_float(w.y >> 16));
+                w[i] = *reinterpret_cast<const uint2*>(static_cast<const __half*>(val ? c.v : c.k) + (val ? c.v_seq : c.k_seq) * s + (val ? c.v_head : c.k_head) * h +
+                                                       (val ? c.v_row : c.k_row) * t + 4 * jr);
             } else {
-                const int nb = c.head_dim / 32, b = j >> 3, jj = j & 7;
-                const uint8_t* base = static_cast<const uint8_t*>(val ? c.v : c.k) + R.seq_bytes * s;
-                const long long row = static_cast<long long>(h) * c.capacity + t;
-                const int at = val ? (jj * nb + b) * 2 : ((jj >> 1) * nb + b) * 4 + (jj & 1) * 2;
-                const unsigned w = *reinterpret_cast<const unsigned short*>(base + row * (c.head_dim / 2) + at);
-                const float2 dm = __half22float2(*reinterpret_cast<const __half2*>(base + R.par_off + (row * nb + b) * 4));
-                f = make_float4(fmaf(dm.x, static_cast<float>(w & 15u), dm.y), fmaf(dm.x, static_cast<float>(w >> 4 & 15u), dm.y),
-                                fmaf(dm.x, static_cast<float>(w >> 8 & 15u), dm.y), fmaf(dm.x, static_cast<float>(w >> 12), dm.y));
+                const uint8_t* plane = static_cast<const uint8_t*>(val ? c.v : c.k) + R.seq_bytes * s;
+                const Q4Place at = q4_place(c, R.par_off, val, h, t, jr);
+                w[i] = make_uint2(*reinterpret_cast<const unsigned short*>(plane + at.codes), *reinterpret_cast<const unsigned*>(plane + at.params));
             }
         }
-        float* dst = (val ? R.v : R.k) + ((static_cast<long long>(s) * R.count + r) * c.kv_heads + h) * c.head_dim + 4 * j;
-        *reinterpret_cast<float4*>(dst) = f;
+#pragma unroll
+        for (int i = 0; i < kRowIter; ++i) {
+            const unsigned r = base + i * per_cta + r0, x = r < rows ? r : r - rows;
+            if (r >= 2 * rows) continue;
+            float4 f;
+            if (BITS == 16) {
+                f = make_float4(half_bits_to_float(w[i].x & 0xFFFFu), half_bits_to_float(w[i].x >> 16), half_bits_to_float(w[i].y & 0xFFFFu), half_bits_to_float(w[i].y >> 16));
+            } else {
+                const float d = half_bits_to_float(w[i].y & 0xFFFFu), m = half_bits_to_float(w[i].y >> 16);
+                f = make_float4(fmaf(d, static_cast<float>(w[i].x & 15u), m), fmaf(d, static_cast<float>(w[i].x >> 4 & 15u), m),
+                                fmaf(d, static_cast<float>(w[i].x >> 8 & 15u), m), fmaf(d, static_cast<float>(w[i].x >> 12), m));
+            }
+            reinterpret_cast<float4*>((r < rows ? R.k : R.v) + (static_cast<size_t>(s) * rows + x) * c.head_dim)[jr] = f;
+        }
     }
 }
 
@@ -167,37 +196,34 @@ __device__ __forceinline__ unsigned weight_key(float w) {
     const unsigned b = __float_as_uint(w);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ int block_scan_exclusive(int v, int* warps, int& total) {  // warps: 33 ints of shared memory
+// Exclusive prefix over the warps of one value per warp (given in every lane); `total` over all.  slots: 33 ints of shared memory.
+__device__ __forceinline__ int warp_prefix(int v, int* slots, int& total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int x = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-    }
     __syncthreads();
-    if (lane == 31) warps[warp] = x;
+    if (lane == 0) slots[warp] = v;
     __syncthreads();
     if (warp == 0) {
-        int t = warps[lane], y = t;
+        const int t = slots[lane];
+        int y = t;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int z = __shfl_up_sync(0xffffffffu, y, o);
             if (lane >= o) y += z;
         }
-        warps[lane] = y - t;
-        if (lane == 31) warps[32] = y;
+        slots[lane] = y - t;
+        if (lane == 31) slots[32] = y;
     }
     __syncthreads();
-    total = warps[32];
-    return warps[warp] + x - v;
+    total = slots[32];
+    return slots[warp];
 }
 __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_constant__ EvictP E) {
     extern __shared__ unsigned keys[];
-    __shared__ int hist[256], scan[33], digit, rest;
+    __shared__ int hist[4][256], slots[33], digit, rest;
     const kcb_kv_cache& c = E.c;
-    const int h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
+    const int h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const size_t sh = static_cast<size_t>(s) * c.kv_heads + h;
+    grid_dependents_may_launch();
     const int n = min(max(0, c.n_keys[s]), c.capacity), keep = E.keep;
     if (n <= keep) {
         if (tid == 0) E.counts[sh] = 0;
@@ -209,21 +235,31 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_con
     const bool held = n <= kSelKeys;
     auto make_key = [&](int t) { return pos[t] >= from ? 0xFFFFFFFFu : weight_key(w[t]); };
     auto key_of = [&](int t) { return held ? keys[t] : make_key(t); };
-    if (held)
-        for (int t = tid; t < n; t += kSelThreads) keys[t] = make_key(t);
+    (&hist[0][0])[tid] = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (int t = tid; t < n; t += kSelThreads) {
+        const unsigned k = make_key(t);
+        if (held) keys[t] = k;
+        atomicAdd(&hist[3][k >> 24], 1);
+    }
+    __syncthreads();
     unsigned prefix = 0, mask = 0;
     int need = keep;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
-        __syncthreads();
-        for (int t = tid; t < n; t += kSelThreads) {
-            const unsigned k = key_of(t);
-            if ((k & mask) == prefix) atomicAdd(&hist[k >> shift & 255u], 1);
+    for (int round = 3; round >= 0; --round) {
+        const int shift = 8 * round;
+        if (round < 3) {
+#pragma unroll 4
+            for (int t = tid; t < n; t += kSelThreads) {
+                const unsigned k = key_of(t);
+                if ((k & mask) == prefix) atomicAdd(&hist[round][k >> shift & 255u], 1);
+            }
+            __syncthreads();
         }
-        __syncthreads();
         if (tid < 32) {  // from the largest digit down: where does the need-th key fall?
-            int sum = 0;
-            for (int i = 0; i < 8; ++i) sum += hist[255 - (tid * 8 + i)];
+            int mine[8], sum = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum += mine[i] = hist[round][255 - (tid * 8 + i)];
             int before = sum;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -232,9 +268,12 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_con
             }
             before -= sum;
             if (before < need && need <= before + sum) {
-                int left = need - before, i = 0;
-                while (left > hist[255 - (tid * 8 + i)]) left -= hist[255 - (tid * 8 + i)], ++i;
-                digit = 255 - (tid * 8 + i), rest = left;
+                int left = need - before;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if (left > 0 && left <= mine[i]) digit = 255 - (tid * 8 + i), rest = left;
+                    left -= mine[i];
+                }
             }
         }
         __syncthreads();
@@ -243,72 +282,92 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_con
         need = rest;
         __syncthreads();
     }
-    // prefix: the keep-th largest key; `need` rows that equal it stay.  Each thread looks after a run of neighbouring slots.
-    const int run = (n + kSelThreads - 1) / kSelThreads, t0 = min(n, tid * run), t1 = min(n, t0 + run);
+    // prefix: the keep-th largest key; `need` rows that equal it stay.  Each warp looks after a run of neighbouring slots, 32 at a
+    // time, so that ballots give the ascending order.
+    const int run = ((n + 31) / 32 + 31) / 32 * 32, t0 = min(n, warp * run), t1 = min(n, t0 + run);
+    const unsigned below = (1u << lane) - 1u;
     int ties = 0, total;
-    for (int t = t0; t < t1; ++t) ties += key_of(t) == prefix;
-    const int tie0 = block_scan_exclusive(ties, scan, total);
+    for (int t = t0; t < t1; t += 32) ties += __popc(__ballot_sync(0xffffffffu, t + lane < t1 && key_of(t + lane) == prefix));
+    const int tie0 = warp_prefix(ties, slots, total);
+    // kept(t) of the 32 slots from t on, as a ballot; moves `tie` on
+    auto kept_of = [&](int t, int& tie) {
+        const unsigned k = t + lane < t1 ? key_of(t + lane) : 0u;
+        const bool in = t + lane < t1, eq = in && k == prefix;
+        const unsigned eqs = __ballot_sync(0xffffffffu, eq);
+        const bool kept = in && (k > prefix || (eq && tie + __popc(eqs & below) < need));
+        tie += __popc(eqs);
+        return __ballot_sync(0xffffffffu, kept);
+    };
     int holes = 0, tails = 0, tie = tie0;
-    for (int t = t0; t < t1; ++t) {
-        const unsigned k = key_of(t);
-        const bool kept = k > prefix || (k == prefix && tie++ < need);
-        if (t < keep) holes += !kept;
-        else tails += kept;
+    for (int t = t0; t < t1; t += 32) {
+        const unsigned kept = kept_of(t, tie), first = __ballot_sync(0xffffffffu, t + lane < min(keep, t1));
+        holes += __popc(first & ~kept), tails += __popc(~first & kept);
     }
-    int hole = block_scan_exclusive(holes, scan, total);
-    int tail = block_scan_exclusive(tails, scan, total);
+    int hole = warp_prefix(holes, slots, total);
+    int tail = warp_prefix(tails, slots, total);
     if (tid == 0) E.counts[sh] = total;
     int2* mv = E.moves + sh * E.max_moves;
     tie = tie0;
-    for (int t = t0; t < t1; ++t) {
-        const unsigned k = key_of(t);
-        const bool kept = k > prefix || (k == prefix && tie++ < need);
-        if (t < keep) {
-            if (!kept) mv[hole++].y = t;
-        } else if (kept) {
-            mv[tail++].x = t;
-        }
+    for (int t = t0; t < t1; t += 32) {
+        const unsigned kept = kept_of(t, tie), first = __ballot_sync(0xffffffffu, t + lane < min(keep, t1));
+        const unsigned ho = first & ~kept, ta = ~first & kept;
+        if (ho >> lane & 1u) mv[hole + __popc(ho & below)].y = t + lane;
+        if (ta >> lane & 1u) mv[tail + __popc(ta & below)].x = t + lane;
+        hole += __popc(ho), tail += __popc(ta);
     }
 }
-// Bounded by memory: every moved row is read and written once.  One warp per row, keys and values 16 (or, for the parameters of
-// narrow heads, 4) bytes a lane.
+// Bounded by memory: every moved row is read and written once.  A warp takes 16 moves at a time, four rows of them in flight.
+// Chunk x of a row: 16 bytes of a key or value (fp16; 4 bits: nibbles, then the parameters four bytes at a time).
+constexpr int kMoveWarps = 8, kMoveRows = 16;
 template <int BITS>
-__global__ void __launch_bounds__(256) kv_move_kernel(const __grid_constant__ EvictP E) {
+__global__ void __launch_bounds__(32 * kMoveWarps) kv_move_kernel(const __grid_constant__ EvictP E) {
     const kcb_kv_cache& c = E.c;
     const int h = blockIdx.y, s = blockIdx.z, lane = threadIdx.x & 31;
     const size_t sh = static_cast<size_t>(s) * c.kv_heads + h;
+    grid_dependency_wait();
     const int count = E.counts[sh];
     if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) c.n_keys[s] = min(max(0, c.n_keys[s]), E.keep);
-    for (int j = blockIdx.x * 8 + (threadIdx.x >> 5); j < count; j += gridDim.x * 8) {
-        const int2 mv = E.moves[sh * E.max_moves + j];
-        if (BITS == 16) {
-            const int chunks = c.head_dim / 8;
-            for (int x = lane; x < 2 * chunks; x += 32) {
-                const bool val = x >= chunks;
-                __half* base = static_cast<__half*>(val ? c.v : c.k) + (val ? c.v_seq : c.k_seq) * s + (val ? c.v_head : c.k_head) * h;
-                const long long row = val ? c.v_row : c.k_row;
-                const int ch = (val ? x - chunks : x) * 8;
-                *reinterpret_cast<uint4*>(base + mv.y * row + ch) = *reinterpret_cast<const uint4*>(base + mv.x * row + ch);
+    const int nb = c.head_dim / 32, chunks = BITS == 16 ? c.head_dim / 8 : 2 * nb;  // per plane
+    for (int j0 = (blockIdx.x * kMoveWarps + (threadIdx.x >> 5)) * kMoveRows; j0 < count; j0 += gridDim.x * kMoveWarps * kMoveRows) {
+        const int rows = min(kMoveRows, count - j0);
+        const int2 mine = E.moves[sh * E.max_moves + j0 + min(lane, rows - 1)];
+        if (lane < rows) {
+            const size_t at = sh * c.capacity;
+            c.positions[at + mine.y] = c.positions[at + mine.x];
+            c.weights[at + mine.y] = c.weights[at + mine.x];
+        }
+        for (int x = lane; x - lane < 2 * chunks; x += 32) {
+            const bool on = x < 2 * chunks, val = on && x >= chunks;
+            const int y = val ? x - chunks : on ? x : 0;
+            const bool wide = BITS == 16 || y < nb;
+            uint8_t* base;
+            size_t row;
+            if (BITS == 16) {
+                base = reinterpret_cast<uint8_t*>(static_cast<__half*>(val ? c.v : c.k) + (val ? c.v_seq : c.k_seq) * s + (val ? c.v_head : c.k_head) * h) + 16 * y;
+                row = 2 * static_cast<size_t>(val ? c.v_row : c.k_row);
+            } else {
+                uint8_t* plane = static_cast<uint8_t*>(val ? c.v : c.k) + E.seq_bytes * s;
+                row = wide ? 16 * nb : 4 * nb;
+                base = plane + (wide ? 0 : E.par_off) + static_cast<size_t>(h) * c.capacity * row + (wide ? 16 * y : 4 * (y - nb));
             }
-        } else {
-            const int nb = c.head_dim / 32;
-            for (int x = lane; x < 4 * nb; x += 32) {  // per plane: nb chunks of 16 bytes of nibbles, nb words of parameters
-                const bool val = x >= 2 * nb;
-                const int y = val ? x - 2 * nb : x;
-                uint8_t* base = static_cast<uint8_t*>(val ? c.v : c.k) + E.seq_bytes * s;
-                const long long from = static_cast<long long>(h) * c.capacity + mv.x, to = static_cast<long long>(h) * c.capacity + mv.y;
-                if (y < nb) {
-                    *reinterpret_cast<uint4*>(base + to * (16 * nb) + y * 16) = *reinterpret_cast<const uint4*>(base + from * (16 * nb) + y * 16);
-                } else {
-                    uint8_t* par = base + E.par_off;
-                    *reinterpret_cast<unsigned*>(par + to * (4 * nb) + (y - nb) * 4) = *reinterpret_cast<const unsigned*>(par + from * (4 * nb) + (y - nb) * 4);
+            for (int j = 0; j < rows; j += 4) {
+                uint4 v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const size_t from = static_cast<size_t>(__shfl_sync(0xffffffffu, mine.x, min(j + i, rows - 1)));
+                    v[i] = make_uint4(0u, 0u, 0u, 0u);
+                    if (!on) continue;
+                    if (wide) v[i] = *reinterpret_cast<const uint4*>(base + from * row);
+                    else v[i].x = *reinterpret_cast<const unsigned*>(base + from * row);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const size_t to = static_cast<size_t>(__shfl_sync(0xffffffffu, mine.y, min(j + i, rows - 1)));
+                    if (!on || j + i >= rows) continue;
+                    if (wide) *reinterpret_cast<uint4*>(base + to * row) = v[i];
+                    else *reinterpret_cast<unsigned*>(base + to * row) = v[i].x;
                 }
             }
-        }
-        if (lane == 0) {
-            const size_t at = sh * c.capacity;
-            c.positions[at + mv.y] = c.positions[at + mv.x];
-            c.weights[at + mv.y] = c.weights[at + mv.x];
         }
     }
 }
@@ -334,18 +393,20 @@ int cache_ok(const kcb_kv_cache* c) {
     return KCB_SUCCESS;
 }
 size_t moves_offset(const kcb_kv_cache* c) { return (static_cast<size_t>(c->n_seqs) * c->kv_heads * 4 + 15) / 16 * 16; }
-unsigned row_blocks(const kcb_kv_cache* c, int rows) {
-    const long long threads = static_cast<long long>(rows) * c->kv_heads * (c->head_dim / 4) * 2;
-    return static_cast<unsigned>(std::min<long long>((threads + 255) / 256, 1 << 20));
+// CTAs of the rows-in and rows-out kernels for one sequence.
+unsigned row_blocks(const kcb_kv_cache* c, int tokens) {
+    const long long rows = 2LL * tokens * c->kv_heads, per_cta = kRowThreads / (c->head_dim / 4) * kRowIter;
+    return static_cast<unsigned>(std::min<long long>((rows + per_cta - 1) / per_cta, 1 << 16));
 }
+constexpr long long kMaxRows = 1LL << 30;  // tokens * kv_heads of one call
 
 // How an attention call is cut: by rows (single tokens) or by tiles of 64 rows (prompts), and into how many ranges of keys.
 struct AttnCut {
     bool tile;
     int row_tiles, nsplit;
-    size_t ml_bytes, o_bytes, final_bytes;
+    size_t ml_bytes, o_bytes, final_bytes, score_bytes;
+    size_t bytes() const { return ml_bytes + o_bytes + final_bytes + score_bytes; }
 };
-constexpr int kRowsMax = 16;
 AttnCut attn_cut(const kcb_kv_cache* c, const kcb_cache_attn* a) {
     AttnCut r{};
     const long long rows = static_cast<long long>(a->n_tokens) * (a->heads / c->kv_heads);
@@ -355,10 +416,13 @@ AttnCut attn_cut(const kcb_kv_cache* c, const kcb_cache_attn* a) {
     const long long want = r.tile ? 2 * kSmCount : 4 * kSmCount, least = r.tile ? 512 : 256;
     long long n = std::min<long long>((want + ctas - 1) / std::max<long long>(ctas, 1), (c->capacity + least - 1) / least);
     r.nsplit = static_cast<int>(std::max<long long>(1, n));
-    const size_t parts = static_cast<size_t>(c->n_seqs) * c->kv_heads * rows * (r.nsplit > 1 ? r.nsplit : 0);
-    r.ml_bytes = (parts * sizeof(float2) + 15) / 16 * 16;
-    r.o_bytes = parts * c->head_dim * sizeof(float);
-    r.final_bytes = a->accumulate ? (static_cast<size_t>(c->n_seqs) * c->kv_heads * rows * sizeof(float2) + 15) / 16 * 16 : 0;
+    // partial sums where keys are split; for weights the rows' final sums (tiles) or every score and the partial sums (rows)
+    const size_t all = static_cast<size_t>(c->n_seqs) * c->kv_heads * rows;
+    const bool weights = a->accumulate != 0;
+    r.ml_bytes = r.nsplit > 1 || (weights && !r.tile) ? (all * r.nsplit * sizeof(float2) + 15) / 16 * 16 : 0;
+    r.o_bytes = r.nsplit > 1 ? all * r.nsplit * c->head_dim * sizeof(float) : 0;
+    r.final_bytes = weights && r.tile ? (all * sizeof(float2) + 15) / 16 * 16 : 0;
+    r.score_bytes = weights && !r.tile ? all * c->capacity * sizeof(float) : 0;
     return r;
 }
 int attn_ok(const kcb_kv_cache* c, const kcb_cache_attn* a) {
@@ -401,29 +465,32 @@ int kcb_cache_append(const kcb_kv_cache* c, const float* k, const float* v, int 
     if (const int e = cache_ok(c); e != KCB_SUCCESS) return e;
     if (!c->n_keys || !k || !v || n_tokens < 0 || token_stride < 0 || seq_stride < 0) return KCB_INVALID_VALUE;
     if (misaligned(k, 16) || misaligned(v, 16) || token_stride % 4 || seq_stride % 4) return KCB_INVALID_POINTER;
+    if (static_cast<long long>(n_tokens) * c->kv_heads > kMaxRows) return KCB_INVALID_VALUE;
     if (n_tokens == 0 || c->n_seqs == 0) return KCB_SUCCESS;
     const auto st = static_cast<cudaStream_t>(stream);
+    const unsigned blocks = row_blocks(c, n_tokens);
+    const bool one = blocks <= 4;  // a step's few rows: one CTA per sequence, which also moves the counts on
     AppendP A{*c, k, v, token_stride, seq_stride, static_cast<long long>(q4_seq_bytes(c->kv_heads, c->head_dim, c->capacity)),
-              static_cast<long long>(q4_param_offset(c->kv_heads, c->head_dim, c->capacity)), n_tokens};
-    const dim3 grid(row_blocks(c, n_tokens), c->n_seqs);
-    if (c->bits == KCB_CACHE_F16) kv_append_rows_kernel<16><<<grid, 256, 0, st>>>(A);
-    else kv_append_rows_kernel<4><<<grid, 256, 0, st>>>(A);
-    if (const int e = launch_status(); e != KCB_SUCCESS) return e;
-    kv_count_kernel<<<(c->n_seqs + 255) / 256, 256, 0, st>>>(c->n_keys, c->next_pos, c->n_seqs, c->capacity, n_tokens);
-    return launch_status();
+              static_cast<long long>(q4_param_offset(c->kv_heads, c->head_dim, c->capacity)), n_tokens, one};
+    const dim3 grid(one ? 1 : blocks, c->n_seqs);
+    if (c->bits == KCB_CACHE_F16) kv_append_rows_kernel<16><<<grid, kRowThreads, 0, st>>>(A);
+    else kv_append_rows_kernel<4><<<grid, kRowThreads, 0, st>>>(A);
+    if (const int e = launch_status(); e != KCB_SUCCESS || one) return e;
+    return launch_dependent(kv_count_kernel, dim3((c->n_seqs + 255) / 256), 256, 0, st, c->n_keys, c->next_pos, c->n_seqs, c->capacity, n_tokens);
 }
 
 int kcb_cache_read(const kcb_kv_cache* c, int first, int count, float* k_out, float* v_out, void* stream) {
     if (const int e = cache_ok(c); e != KCB_SUCCESS) return e;
     if (!k_out || !v_out || first < 0 || count < 0 || first > c->capacity - count) return KCB_INVALID_VALUE;
     if (misaligned(k_out, 16) || misaligned(v_out, 16)) return KCB_INVALID_POINTER;
+    if (static_cast<long long>(count) * c->kv_heads > kMaxRows) return KCB_INVALID_VALUE;
     if (count == 0 || c->n_seqs == 0) return KCB_SUCCESS;
     const auto st = static_cast<cudaStream_t>(stream);
     ReadP R{*c, k_out, v_out, static_cast<long long>(q4_seq_bytes(c->kv_heads, c->head_dim, c->capacity)),
             static_cast<long long>(q4_param_offset(c->kv_heads, c->head_dim, c->capacity)), first, count};
     const dim3 grid(row_blocks(c, count), c->n_seqs);
-    if (c->bits == KCB_CACHE_F16) kv_read_rows_kernel<16><<<grid, 256, 0, st>>>(R);
-    else kv_read_rows_kernel<4><<<grid, 256, 0, st>>>(R);
+    if (c->bits == KCB_CACHE_F16) kv_read_rows_kernel<16><<<grid, kRowThreads, 0, st>>>(R);
+    else kv_read_rows_kernel<4><<<grid, kRowThreads, 0, st>>>(R);
     return launch_status();
 }
 
@@ -446,16 +513,15 @@ int kcb_cache_evict(const kcb_kv_cache* c, int keep, int recent, void* workspace
     if (!raise_dynamic_smem(kv_select_kernel, kSelKeys * 4, raised)) return KCB_LAUNCH_FAILURE;
     kv_select_kernel<<<dim3(c->kv_heads, c->n_seqs), kSelThreads, std::min(c->capacity, kSelKeys) * 4, st>>>(E);
     if (const int e = launch_status(); e != KCB_SUCCESS) return e;
-    const dim3 grid(std::min((E.max_moves + 7) / 8, 1024), c->kv_heads, c->n_seqs);
-    if (c->bits == KCB_CACHE_F16) kv_move_kernel<16><<<grid, 256, 0, st>>>(E);
-    else kv_move_kernel<4><<<grid, 256, 0, st>>>(E);
-    return launch_status();
+    constexpr int per_cta = kMoveWarps * kMoveRows;
+    const dim3 grid(std::min((E.max_moves + per_cta - 1) / per_cta, 1024), c->kv_heads, c->n_seqs);
+    return c->bits == KCB_CACHE_F16 ? launch_dependent(kv_move_kernel<16>, grid, 32 * kMoveWarps, 0, st, E)
+                                    : launch_dependent(kv_move_kernel<4>, grid, 32 * kMoveWarps, 0, st, E);
 }
 
 size_t kcb_cache_attention_workspace_bytes(const kcb_kv_cache* c, const kcb_cache_attn* a) {
     if (attn_ok(c, a) != KCB_SUCCESS || a->n_tokens == 0 || c->n_seqs == 0) return 0;
-    const AttnCut cut = attn_cut(c, a);
-    return cut.ml_bytes + cut.o_bytes + cut.final_bytes;
+    return attn_cut(c, a).bytes();
 }
 
 int kcb_cache_attention(const kcb_kv_cache* c, const kcb_cache_attn* a, const float* q, float* out, void* workspace, size_t workspace_bytes, void* stream) {
@@ -464,7 +530,7 @@ int kcb_cache_attention(const kcb_kv_cache* c, const kcb_cache_attn* a, const fl
     if (misaligned(q, 16) || misaligned(out, 16)) return KCB_INVALID_POINTER;
     if (a->n_tokens == 0 || c->n_seqs == 0) return KCB_SUCCESS;
     const AttnCut cut = attn_cut(c, a);
-    const size_t need = cut.ml_bytes + cut.o_bytes + cut.final_bytes;
+    const size_t need = cut.bytes();
     if (need && (!workspace || workspace_bytes < need)) return KCB_INVALID_VALUE;
     if (misaligned(workspace, 16)) return KCB_INVALID_POINTER;
     AttnP P{};
@@ -488,7 +554,9 @@ int kcb_cache_attention(const kcb_kv_cache* c, const kcb_cache_attn* a, const fl
     P.nsplit = cut.nsplit, P.row_tiles = cut.row_tiles;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     P.part_ml = reinterpret_cast<float2*>(ws), P.part_o = reinterpret_cast<float*>(ws + cut.ml_bytes);
-    P.final_ml = a->accumulate ? reinterpret_cast<float2*>(ws + cut.ml_bytes + cut.o_bytes) : nullptr;
+    ws += cut.ml_bytes + cut.o_bytes;
+    P.final_ml = cut.final_bytes ? reinterpret_cast<float2*>(ws) : nullptr;
+    P.scores = cut.score_bytes ? reinterpret_cast<float*>(ws) : nullptr;
     const bool general = a->softcap > 0.0f || a->max_bias > 0.0f || c->positions || a->q_pos || a->q_doc || a->mask || a->prefix;
     const auto st = static_cast<cudaStream_t>(stream);
     return attn_launch_bits(P, c->bits, c->head_dim, general, cut.tile, st);

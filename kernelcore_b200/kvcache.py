@@ -36,16 +36,18 @@ _L.kcb_cache_attention_workspace_bytes.argtypes = [C.POINTER(_Cache), C.POINTER(
 _L.kcb_cache_attention.argtypes = [C.POINTER(_Cache), C.POINTER(_Attn), C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
 
 
-def _launch(what: str, device: torch.device, *args) -> None:
-    """Calls kcb_<what>(*args, stream) with the tensors' device current, on the stream that is current there."""
-    fn = getattr(_L, what)
+_stream = torch._C._cuda_getCurrentRawStream  # of a device index; the tensor-free form of torch.cuda.current_stream
+
+
+def _launch(fn, device: torch.device, *args) -> None:
+    """fn(*args, stream) with the tensors' device current, on the stream that is current there."""
     if torch.cuda.current_device() == device.index:
-        status = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+        status = fn(*args, _stream(device.index))
     else:
         with torch.cuda.device(device):
-            status = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+            status = fn(*args, _stream(device.index))
     if status:
-        lib.check(status, what)
+        lib.check(status, fn.__name__)
 
 
 def _on(t: torch.Tensor, dtype, shape, what: str, device) -> int:
@@ -90,7 +92,7 @@ class KVCache:
         self.k, self.v, self.n_keys, self.next_pos, self.positions, self.weights = k, v, n_keys, next_pos, positions, weights
         self.bits, self.n_seqs, self.kv_heads, self.head_dim, self.capacity = bits, c.n_seqs, kv_heads, head_dim, capacity
         self.struct, self._ref = c, C.byref(c)
-        self._evict_ws: dict[int, torch.Tensor] = {}
+        self._evict_ws: dict[int, tuple] = {}  # by `keep`, kept: captured graphs go on using theirs
 
     @classmethod
     def empty(cls, n_seqs: int, kv_heads: int, head_dim: int, capacity: int, bits: int = 16, evictable: bool = False, device="cuda") -> "KVCache":
@@ -110,15 +112,14 @@ class KVCache:
     def append(self, k: torch.Tensor, v: torch.Tensor) -> None:
         """New rows behind those in use: fp32 [n_seqs][n_tokens][kv_heads][head_dim], heads and channels contiguous, k and v
         with the same strides (slices of one q|k|v product are)."""
-        for name, t in (("k", k), ("v", v)):
-            if t.dtype != torch.float32 or t.dim() != 4 or t.shape[0] != self.n_seqs or tuple(t.shape[2:]) != (self.kv_heads, self.head_dim) or t.shape != k.shape or \
-                    t.stride()[:2] != k.stride()[:2] or t.stride(3) != 1 or (self.kv_heads > 1 and t.stride(2) != self.head_dim) or t.device != self.device:
-                raise ValueError(f"{name}: fp32 [{self.n_seqs}][n_tokens][{self.kv_heads}][{self.head_dim}] on {self.device} is needed, got {t.dtype} "
-                                 f"{tuple(t.shape)} with strides {t.stride()} on {t.device}")
-        if not k.numel():
-            return
-        tok, seq = k.stride(1), k.stride(0)
-        _launch("kcb_cache_append", self.device, self._ref, k.data_ptr(), v.data_ptr(), k.shape[1], tok, seq)
+        shape, stride = k.shape, k.stride()
+        if len(shape) != 4 or shape[0] != self.n_seqs or shape[2] != self.kv_heads or shape[3] != self.head_dim or stride[3] != 1 or v.shape != shape or \
+                v.stride() != stride or (self.kv_heads > 1 and stride[2] != self.head_dim) or k.dtype != torch.float32 or v.dtype != torch.float32 or \
+                k.device != self.device or v.device != self.device:
+            raise ValueError(f"k, v: fp32 [{self.n_seqs}][n_tokens][{self.kv_heads}][{self.head_dim}] on {self.device} with the same strides are needed, got " +
+                             " and ".join(f"{t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}" for t in (k, v)))
+        if shape[1] and shape[0]:
+            _launch(_L.kcb_cache_append, self.device, self._ref, k.data_ptr(), v.data_ptr(), shape[1], stride[1], stride[0])
 
     def read(self, first: int, count: int) -> tuple[torch.Tensor, torch.Tensor]:
         """Slots first .. first + count - 1 as fp32 [n_seqs][count][kv_heads][head_dim], zeros where no row is in use."""
@@ -126,16 +127,17 @@ class KVCache:
             raise ValueError(f"slots {first} .. {first + count - 1} of {self.capacity}")
         k, v = (torch.empty(self.n_seqs, count, self.kv_heads, self.head_dim, device=self.device) for _ in range(2))
         if k.numel():
-            _launch("kcb_cache_read", self.device, self._ref, first, count, k.data_ptr(), v.data_ptr())
+            _launch(_L.kcb_cache_read, self.device, self._ref, first, count, k.data_ptr(), v.data_ptr())
         return k, v
 
     def evict(self, keep: int, recent: int) -> None:
         """Sequences that hold more than `keep` rows drop the least attended ones (never one of the `recent` newest tokens)."""
         ws = self._evict_ws.get(keep)
         if ws is None:
-            ws = torch.empty(max(16, _L.kcb_cache_evict_workspace_bytes(self._ref, keep)), dtype=torch.uint8, device=self.device)
-            self._evict_ws = {keep: ws}
-        _launch("kcb_cache_evict", self.device, self._ref, keep, recent, ws.data_ptr(), ws.numel())
+            n = max(16, _L.kcb_cache_evict_workspace_bytes(self._ref, keep))
+            buf = torch.empty(n, dtype=torch.uint8, device=self.device)
+            ws = self._evict_ws[keep] = (buf, buf.data_ptr(), n)
+        _launch(_L.kcb_cache_evict, self.device, self._ref, keep, recent, ws[1], ws[2])
 
 
 class Attention:
@@ -158,7 +160,8 @@ class Attention:
             a.mask, a.mask_seq, a.mask_token = mask.data_ptr(), mask.stride(0), mask.stride(1)
         self.cache, self.struct, self._ref = cache, a, C.byref(a)
         self._keep = (prefix, q_pos, q_doc, k_doc, mask)
-        self.shape = (S, n_tokens, heads, cache.head_dim)
+        self.shape = torch.Size((S, n_tokens, heads, cache.head_dim))
+        self._empty, self._strides = self.shape.numel() == 0, None
         n = _L.kcb_cache_attention_workspace_bytes(cache._ref, self._ref)
         self.workspace = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
         self._ws = (self.workspace.data_ptr(), n) if n else (None, 0)
@@ -168,13 +171,17 @@ class Attention:
         dev = self.cache.device
         if out is None:
             out = torch.empty(self.shape, device=dev)
-        a = self.struct
-        for name, t in (("q", q), ("out", out)):
-            if t.dtype != torch.float32 or t.shape != self.shape or t.stride(3) != 1 or t.device != dev:
-                raise ValueError(f"{name}: fp32 {self.shape} with contiguous channels on {dev} is needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
-        if not q.numel():
+        qs, os = q.stride(), out.stride()
+        if q.shape != self.shape or out.shape != self.shape or q.dtype != torch.float32 or out.dtype != torch.float32 or qs[3] != 1 or os[3] != 1 or \
+                q.device != dev or out.device != dev:
+            raise ValueError(f"q, out: fp32 {tuple(self.shape)} with contiguous channels on {dev} are needed, got " +
+                             " and ".join(f"{t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}" for t in (q, out)))
+        if self._strides != (qs, os):
+            a = self.struct
+            a.q_seq, a.q_token, a.q_head, _ = qs
+            a.out_seq, a.out_token, a.out_head, _ = os
+            self._strides = (qs, os)
+        if self._empty:
             return out
-        a.q_seq, a.q_token, a.q_head = q.stride()[:3]
-        a.out_seq, a.out_token, a.out_head = out.stride()[:3]
-        _launch("kcb_cache_attention", dev, self.cache._ref, self._ref, q.data_ptr(), out.data_ptr(), *self._ws)
+        _launch(_L.kcb_cache_attention, dev, self.cache._ref, self._ref, q.data_ptr(), out.data_ptr(), *self._ws)
         return out
