@@ -3,11 +3,16 @@
 #ifdef KV_BITS
 
 #include "kv_attention.cuh"
+#include "kv_attention_tc.cuh"
 
 namespace kcb {
 template <>
-int attn_launch<KV_BITS, KV_DIM>(const AttnP& P, bool general, bool tile, cudaStream_t st) {
-    return attn_launch_kernels<KV_DIM, KV_BITS>(P, general, tile, st);
+int attn_launch<KV_BITS, KV_DIM>(const AttnP& P, bool general, AttnKernel which, cudaStream_t st) {
+    return attn_launch_kernels<KV_DIM, KV_BITS>(P, general, which, st);
+}
+template <>
+unsigned attn_timeouts_of<KV_BITS, KV_DIM>() {
+    return attn_timeouts_here();
 }
 }  // namespace kcb
 
@@ -18,19 +23,20 @@ int attn_launch<KV_BITS, KV_DIM>(const AttnP& P, bool general, bool tile, cudaSt
 
 namespace kcb {
 template <int BITS>
-static int attn_launch_dim(const AttnP& P, int head_dim, bool general, bool tile, cudaStream_t st) {
+static int attn_launch_dim(const AttnP& P, int head_dim, bool general, AttnKernel which, cudaStream_t st) {
     switch (head_dim) {
-    case 32: return attn_launch<BITS, 32>(P, general, tile, st);
-    case 64: return attn_launch<BITS, 64>(P, general, tile, st);
-    case 96: return attn_launch<BITS, 96>(P, general, tile, st);
-    case 128: return attn_launch<BITS, 128>(P, general, tile, st);
-    case 256: return attn_launch<BITS, 256>(P, general, tile, st);
+    case 32: return attn_launch<BITS, 32>(P, general, which, st);
+    case 64: return attn_launch<BITS, 64>(P, general, which, st);
+    case 96: return attn_launch<BITS, 96>(P, general, which, st);
+    case 128: return attn_launch<BITS, 128>(P, general, which, st);
+    case 256: return attn_launch<BITS, 256>(P, general, which, st);
     }
     return KCB_UNSUPPORTED_OPERATION;
 }
-int attn_launch_bits(const AttnP& P, int bits, int head_dim, bool general, bool tile, cudaStream_t st) {
-    return bits == KCB_CACHE_F16 ? attn_launch_dim<16>(P, head_dim, general, tile, st) : attn_launch_dim<4>(P, head_dim, general, tile, st);
+int attn_launch_bits(const AttnP& P, int bits, int head_dim, bool general, AttnKernel which, cudaStream_t st) {
+    return bits == KCB_CACHE_F16 ? attn_launch_dim<16>(P, head_dim, general, which, st) : attn_launch_dim<4>(P, head_dim, general, which, st);
 }
+unsigned attn_timeouts() { return attn_timeouts_of<16, 64>() + attn_timeouts_of<16, 128>() + attn_timeouts_of<4, 64>() + attn_timeouts_of<4, 128>(); }
 }  // namespace kcb
 
 #endif

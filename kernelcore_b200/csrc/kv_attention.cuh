@@ -134,20 +134,18 @@ __device__ __forceinline__ void row_scale(float amax, float& up, float& down) {
 }
 // tanh to fp32 accuracy.  Below 0.55 the odd power series (coefficients B_2n 2^2n (2^2n - 1) / (2n)!, truncated after
 // u^15: 2e-8 relative there); above it the library's function.  Capped scores are mostly small against their cap.
-__device__ __forceinline__ float tanh_acc(float u) {
+__device__ __forceinline__ float tanh_series(float u) {
     const float w = u * u;
-    if (w < 0.3025f) {
-        float r = -1.4558344e-3f;
-        r = fmaf(r, w, 3.5921280e-3f);
-        r = fmaf(r, w, -8.8632355e-3f);
-        r = fmaf(r, w, 2.1869488e-2f);
-        r = fmaf(r, w, -5.3968254e-2f);
-        r = fmaf(r, w, 1.3333333e-1f);
-        r = fmaf(r, w, -3.3333333e-1f);
-        return fmaf(u * w, r, u);
-    }
-    return tanhf(u);
+    float r = -1.4558344e-3f;
+    r = fmaf(r, w, 3.5921280e-3f);
+    r = fmaf(r, w, -8.8632355e-3f);
+    r = fmaf(r, w, 2.1869488e-2f);
+    r = fmaf(r, w, -5.3968254e-2f);
+    r = fmaf(r, w, 1.3333333e-1f);
+    r = fmaf(r, w, -3.3333333e-1f);
+    return fmaf(u * w, r, u);
 }
+__device__ __forceinline__ float tanh_acc(float u) { return fabsf(u) < 0.55f ? tanh_series(u) : tanhf(u); }
 // Values that are not finite, of which a product with a zero weight would make NaN: found 16 bytes at a time, added to a row
 // that sees them, and cleared from a tile.
 __device__ __forceinline__ bool not_finite2(unsigned w) { return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u; }
@@ -232,6 +230,53 @@ __device__ __forceinline__ float general_score(const AttnP& P, float z, const Ro
     }
     return see ? y : -INFINITY;
 }
+
+// Which key tiles of [begin, end) hold a document of the query tokens tok0 .. tok1: a bitmap in shared memory, a bit per 2^k tiles
+// with k so large that kDocBits bits are enough.
+constexpr int kDocBits = 8192;
+template <int TK>
+struct DocTiles {
+    uint32_t* bits;
+    int nt;
+    __device__ __forceinline__ int shift() const { return nt <= kDocBits ? 0 : 32 - __clz((nt - 1) / kDocBits); }
+    __device__ __forceinline__ void clear(int tid, int threads) const {
+        for (int i = tid; i < kDocBits / 32; i += threads) bits[i] = 0u;
+    }
+    __device__ __forceinline__ void find(const AttnP& P, int s, int tok0, int tok1, int begin, int end, int warp, int warps, int lane) const {
+        int lo = INT32_MAX, hi = INT32_MIN;
+        for (int t = tok0 + lane; t <= tok1; t += 32) {
+            const int d = P.q_doc[static_cast<size_t>(s) * P.n_tokens + t];
+            lo = min(lo, d), hi = max(hi, d);
+        }
+        lo = __reduce_min_sync(0xffffffffu, lo), hi = __reduce_max_sync(0xffffffffu, hi);
+        const int* kd = P.k_doc + static_cast<size_t>(s) * P.cap;
+        const int sh = shift();
+        constexpr int kAhead = 8, kPer = TK / 32;  // tiles whose documents are requested at once
+        for (int i0 = warp; i0 < nt; i0 += warps * kAhead) {
+            int d[kAhead][kPer];
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+                for (int k = 0; k < kPer; ++k) {
+                    const int t = begin + (i0 + a * warps) * TK + k * 32 + lane;
+                    d[a][k] = i0 + a * warps < nt && t < end ? kd[t] : (lo > INT32_MIN ? lo - 1 : hi + 1);
+                }
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a) {
+                bool any = false;
+#pragma unroll
+                for (int k = 0; k < kPer; ++k) any = any || (d[a][k] >= lo && d[a][k] <= hi);
+                const int i = (i0 + a * warps) >> sh;
+                if (__any_sync(0xffffffffu, any) && lane == 0) atomicOr(&bits[i / 32], 1u << (i % 32));
+            }
+        }
+    }
+    __device__ __forceinline__ int next(int i) const {  // the wanted tile behind tile i, nt if there is none
+        const int sh = shift();
+        for (++i; i < nt && !(bits[(i >> sh) / 32] >> ((i >> sh) % 32) & 1u); ++i) {}
+        return i;
+    }
+};
 
 // ---- cache tiles in shared memory -----------------------------------------------------------------------------------
 // fp16: rows of D halves, padded by 16 bytes so that the eight rows of an ldmatrix fall into different banks.
@@ -892,7 +937,8 @@ struct TileCfg {
     static constexpr int kPlane = Tile<D, FMT>::bytes(kKeys);
     static constexpr int kOffKv = QTile<D>::kBytes;
     static constexpr int kOffBits = kOffKv + 4 * kPlane;  // bitmap of the tiles that hold a document of these rows
-    static int smem(int tiles) { return kOffBits + (tiles + 31) / 32 * 4; }
+    static constexpr int kSmem = kOffBits + kDocBits / 8;
+    static_assert(kSmem <= kMaxSmem);
 };
 
 template <int D, int FMT, bool GEN>
@@ -917,36 +963,16 @@ __global__ void __launch_bounds__(128) attn_tile_kernel(const __grid_constant__ 
         end = max(begin, min(end, max(prefix, row_pos(P, s, n, tok1) + 1)));
     const int nt = (end - begin + TK - 1) / TK;
 
-    uint32_t* bits = reinterpret_cast<uint32_t*>(sm + C::kOffBits);
     const bool docs = GEN && P.q_doc != nullptr;
+    const DocTiles<TK> doc_tiles{reinterpret_cast<uint32_t*>(sm + C::kOffBits), nt};
     if (docs) {
-        int lo = INT32_MAX, hi = INT32_MIN;
-        for (int t = tok0 + lane; t <= tok1; t += 32) {
-            const int d = P.q_doc[static_cast<size_t>(s) * P.n_tokens + t];
-            lo = min(lo, d), hi = max(hi, d);
-        }
-        lo = __reduce_min_sync(0xffffffffu, lo), hi = __reduce_max_sync(0xffffffffu, hi);
-        for (int i = tid; i < (nt + 31) / 32; i += 128) bits[i] = 0u;
+        doc_tiles.clear(tid, 128);
         __syncthreads();
-        for (int i = warp; i < nt; i += 4) {
-            bool any = false;
-            for (int k = lane; k < TK; k += 32) {
-                const int t = begin + i * TK + k;
-                if (t < end) {
-                    const int d = P.k_doc[static_cast<size_t>(s) * P.cap + t];
-                    any = any || (d >= lo && d <= hi);
-                }
-            }
-            if (__any_sync(0xffffffffu, any) && lane == 0) atomicOr(&bits[i / 32], 1u << (i % 32));
-        }
+        doc_tiles.find(P, s, tok0, tok1, begin, end, warp, 4, lane);
     }
     load_q_tile<D, FMT>(P, s, kvh, row0, sm, tid);
     __syncthreads();
-    auto next = [&](int i) {
-        if (docs)
-            while (i < nt && !(bits[i / 32] >> (i % 32) & 1u)) ++i;
-        return i;
-    };
+    auto next = [&](int i) { return docs ? doc_tiles.next(i) : i + 1; };  // the tile behind tile i that is wanted
     auto fetch = [&](int i, int stage) {
         if (i < nt) {
             const uint32_t dst = smem_u32(sm) + C::kOffKv + stage * 2 * C::kPlane;
@@ -977,10 +1003,10 @@ __global__ void __launch_bounds__(128) attn_tile_kernel(const __grid_constant__ 
 #pragma unroll
     for (int b = 0; b < (FMT == 16 ? 1 : NB); ++b) oma[b] = omb[b] = 0.0f;
 
-    int cur = next(0), stage = 0;
+    int cur = next(-1), stage = 0;
     fetch(cur, 0);
     while (cur < nt) {
-        const int nxt = next(cur + 1);
+        const int nxt = next(cur);
         fetch(nxt, stage ^ 1);
         cp_wait<1>();
         const uint8_t* kt = sm + C::kOffKv + stage * 2 * C::kPlane;
@@ -1257,23 +1283,27 @@ __global__ void __launch_bounds__(128) attn_weights_kernel(const __grid_constant
 }
 
 // ---- launches --------------------------------------------------------------------------------------------------------------------
+// kv_attention_tc.cuh
 template <int D, int FMT>
-int attn_launch_kernels(const AttnP& P, bool general, bool tile, cudaStream_t st) {
-    int smem;
-    if (tile) {
-        smem = TileCfg<D, FMT>::smem(P.q_doc ? (P.cap + TileCfg<D, FMT>::kKeys - 1) / TileCfg<D, FMT>::kKeys : 0);
-        if (smem > kMaxSmem) return KCB_UNSUPPORTED_OPERATION;
+int attn_launch_tc(const AttnP& P, bool general, cudaStream_t st);
+
+template <int D, int FMT>
+int attn_launch_kernels(const AttnP& P, bool general, AttnKernel which, cudaStream_t st) {
+    if (which == AttnKernel::tc) {
+        if (const int e = attn_launch_tc<D, FMT>(P, general, st); e != KCB_SUCCESS) return e;
+    } else if (which == AttnKernel::tile) {
+        constexpr int smem = TileCfg<D, FMT>::kSmem;
         static PerDeviceFlag raised[2];
         const dim3 grid(P.row_tiles * P.nsplit, P.kv_heads, P.n_seqs);
         if (general) {
-            if (!raise_dynamic_smem(attn_tile_kernel<D, FMT, true>, kMaxSmem, raised[0])) return KCB_LAUNCH_FAILURE;
+            if (!raise_dynamic_smem(attn_tile_kernel<D, FMT, true>, smem, raised[0])) return KCB_LAUNCH_FAILURE;
             attn_tile_kernel<D, FMT, true><<<grid, 128, smem, st>>>(P);
         } else {
-            if (!raise_dynamic_smem(attn_tile_kernel<D, FMT, false>, kMaxSmem, raised[1])) return KCB_LAUNCH_FAILURE;
+            if (!raise_dynamic_smem(attn_tile_kernel<D, FMT, false>, smem, raised[1])) return KCB_LAUNCH_FAILURE;
             attn_tile_kernel<D, FMT, false><<<grid, 128, smem, st>>>(P);
         }
     } else {
-        smem = RowsCfg<D, FMT>::kSmem;
+        constexpr int smem = RowsCfg<D, FMT>::kSmem;
         static PerDeviceFlag raised[2];
         const dim3 grid(P.nsplit, P.kv_heads * P.row_tiles, P.n_seqs);
         if (general) {

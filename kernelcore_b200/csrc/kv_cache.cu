@@ -402,27 +402,28 @@ constexpr long long kMaxRows = 1LL << 30;  // tokens * kv_heads of one call
 
 // How an attention call is cut: by rows (single tokens) or by tiles of 64 rows (prompts), and into how many ranges of keys.
 struct AttnCut {
-    bool tile;
+    AttnKernel which;
     int row_tiles, nsplit;
     size_t ml_bytes, o_bytes, final_bytes, score_bytes;
     size_t bytes() const { return ml_bytes + o_bytes + final_bytes + score_bytes; }
 };
+constexpr int kTcRows = 96;  // query rows per kv head from which the tcgen05 kernel is taken
 AttnCut attn_cut(const kcb_kv_cache* c, const kcb_cache_attn* a) {
     AttnCut r{};
     const long long rows = static_cast<long long>(a->n_tokens) * (a->heads / c->kv_heads);
-    r.tile = rows > kRowsMax;
-    r.row_tiles = static_cast<int>(r.tile ? (rows + 63) / 64 : (rows + 7) / 8);
+    r.which = rows <= kRowsMax ? AttnKernel::rows : rows >= kTcRows && (c->head_dim == 64 || c->head_dim == 128) ? AttnKernel::tc : AttnKernel::tile;
+    const int per = r.which == AttnKernel::rows ? 8 : r.which == AttnKernel::tile ? 64 : 128;
+    r.row_tiles = static_cast<int>((rows + per - 1) / per);
     const long long ctas = static_cast<long long>(c->n_seqs) * c->kv_heads * r.row_tiles;
-    const long long want = r.tile ? 2 * kSmCount : 4 * kSmCount, least = r.tile ? 512 : 256;
-    long long n = std::min<long long>((want + ctas - 1) / std::max<long long>(ctas, 1), (c->capacity + least - 1) / least);
-    r.nsplit = static_cast<int>(std::max<long long>(1, n));
+    const long long want = (r.which == AttnKernel::rows ? 4 : r.which == AttnKernel::tile ? 2 : 1) * kSmCount, least = r.which == AttnKernel::rows ? 256 : 512;
+    r.nsplit = static_cast<int>(std::max<long long>(1, std::min<long long>(want / std::max<long long>(ctas, 1), (c->capacity + least - 1) / least)));
     // partial sums where keys are split; for weights the rows' final sums (tiles) or every score and the partial sums (rows)
     const size_t all = static_cast<size_t>(c->n_seqs) * c->kv_heads * rows;
     const bool weights = a->accumulate != 0;
-    r.ml_bytes = r.nsplit > 1 || (weights && !r.tile) ? (all * r.nsplit * sizeof(float2) + 15) / 16 * 16 : 0;
+    r.ml_bytes = r.nsplit > 1 || (weights && r.which == AttnKernel::rows) ? (all * r.nsplit * sizeof(float2) + 15) / 16 * 16 : 0;
     r.o_bytes = r.nsplit > 1 ? all * r.nsplit * c->head_dim * sizeof(float) : 0;
-    r.final_bytes = weights && r.tile ? (all * sizeof(float2) + 15) / 16 * 16 : 0;
-    r.score_bytes = weights && !r.tile ? all * c->capacity * sizeof(float) : 0;
+    r.final_bytes = weights && r.which != AttnKernel::rows ? (all * sizeof(float2) + 15) / 16 * 16 : 0;
+    r.score_bytes = weights && r.which == AttnKernel::rows ? all * c->capacity * sizeof(float) : 0;
     return r;
 }
 int attn_ok(const kcb_kv_cache* c, const kcb_cache_attn* a) {
@@ -559,7 +560,7 @@ int kcb_cache_attention(const kcb_kv_cache* c, const kcb_cache_attn* a, const fl
     P.scores = cut.score_bytes ? reinterpret_cast<float*>(ws) : nullptr;
     const bool general = a->softcap > 0.0f || a->max_bias > 0.0f || c->positions || a->q_pos || a->q_doc || a->mask || a->prefix;
     const auto st = static_cast<cudaStream_t>(stream);
-    return attn_launch_bits(P, c->bits, c->head_dim, general, cut.tile, st);
+    return attn_launch_bits(P, c->bits, c->head_dim, general, cut.which, st);
 }
 
 }  // extern "C"

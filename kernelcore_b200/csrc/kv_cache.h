@@ -13,9 +13,13 @@ constexpr int kMaxSmem = 227 * 1024;  // dynamic shared memory a CTA may ask for
 
 struct AttnP;
 // One instance per cache format and head dimension (kv_attention.cu), and the choice among them.
+enum class AttnKernel { rows, tile, tc };
 template <int BITS, int D>
-int attn_launch(const AttnP& P, bool general, bool tile, cudaStream_t st);
-int attn_launch_bits(const AttnP& P, int bits, int head_dim, bool general, bool tile, cudaStream_t st);
+int attn_launch(const AttnP& P, bool general, AttnKernel which, cudaStream_t st);
+template <int BITS, int D>
+unsigned attn_timeouts_of();
+int attn_launch_bits(const AttnP& P, int bits, int head_dim, bool general, AttnKernel which, cudaStream_t st);
+unsigned attn_timeouts();  // bounded waits of the attention kernels that expired since load; synchronous
 
 // Bytes of one sequence's keys (or values) in the 4-bit format, and where its parameter plane begins.
 inline size_t q4_param_offset(int kv_heads, int head_dim, int capacity) { return static_cast<size_t>(kv_heads) * capacity * (head_dim / 2); }

@@ -124,7 +124,10 @@ SHAPES = [  # S, N, heads, kv heads, D, capacity, rows in use
     (1, 1, 1, 1, 32, 1, [1]), (1, 1, 4, 1, 64, 17, [16]), (2, 1, 12, 4, 64, 77, [77, 0]), (3, 1, 6, 2, 128, 300, [300, 1, 129]), (1, 1, 10, 2, 96, 65, [64]),
     (1, 1, 16, 1, 256, 50, [33]), (1, 2, 32, 8, 128, 1000, [999]), (2, 5, 3, 3, 32, 40, [40, 3]), (1, 1, 24, 1, 64, 700, [700]),
     (1, 17, 4, 4, 128, 64, [64]), (2, 33, 8, 2, 64, 130, [129, 40]), (1, 65, 2, 1, 96, 65, [65]), (1, 40, 6, 2, 256, 100, [90]), (1, 130, 5, 1, 32, 300, [290]),
-    (1, 100, 8, 8, 128, 1300, [1222]), (1, 16, 8, 4, 64, 5000, [4801])]
+    (1, 100, 8, 8, 128, 1300, [1222]), (1, 16, 8, 4, 64, 5000, [4801]),
+    # 96 rows per kv head and more at D = 64 and 128: the tcgen05 kernel (one row tile and several, one key tile, few, many, split)
+    (1, 96, 1, 1, 64, 96, [96]), (1, 97, 3, 3, 128, 97, [97]), (2, 130, 4, 2, 128, 150, [150, 131]), (1, 300, 6, 2, 64, 700, [650]), (1, 128, 1, 1, 128, 3000, [2999]),
+    (3, 64, 4, 2, 64, 64, [64, 0, 1]), (1, 1000, 2, 2, 128, 1000, [1000]), (1, 50, 16, 2, 128, 63, [63])]
 
 
 @pytest.mark.parametrize("bits", [16, 4])
@@ -179,17 +182,17 @@ def test_attention_forms(bits, N, H, Hkv, D, cap, form):
 
 @pytest.mark.parametrize("bits", [16, 4])
 @pytest.mark.parametrize("size", [1e-4, 1e-2, 30.0, 3000.0])
-@pytest.mark.parametrize("N", [1, 24])
+@pytest.mark.parametrize("N", [1, 24, 150])
 def test_attention_of_small_and_large_values(bits, size, N):
     """Values (and, scaled back, keys) of every magnitude that fp16 holds: the probabilities' split must not lose them."""
-    c, k, v, gen = filled(bits, 1, 200, 2, 64, [200], seed=11, size=size)
+    c, k, v, gen = filled(bits, 1, 200, 2, 64, [200], seed=11, size=size)   # (96 rows and more: the tcgen05 kernel)
     q = torch.randn(1, N, 4, 64, generator=gen, device="cuda")
     check(c, k, v, q, N, 4, scale=0.125 / size)
     check(c, k, v, 1e-6 * q, N, 4, scale=1e6 * 0.125 / size)
 
 
 @pytest.mark.parametrize("bits", [16, 4])
-@pytest.mark.parametrize("N", [1, 40])
+@pytest.mark.parametrize("N", [1, 40, 130])
 def test_what_is_hidden_never_reaches_an_output(bits, N):
     """Garbage behind the rows in use and in hidden slots: infinities and NaN, as keys, values or 4-bit scales."""
     S, H, Hkv, D, cap = 1, 4, 2, 128, 200
@@ -223,7 +226,7 @@ def test_what_is_hidden_never_reaches_an_output(bits, N):
     assert torch.equal(kvcache.Attention(c2, n_tokens=N, heads=H)(q2), plain)
 
 
-@pytest.mark.parametrize("N", [4, 40])
+@pytest.mark.parametrize("N", [4, 40, 80])
 def test_an_infinite_value_reaches_those_who_see_it(N):
     """Causal: the newest slot holds an infinity and a NaN; the last token sees them, the ones before it do not."""
     c, k, v, gen = filled(16, 1, 100, 1, 64, [100], seed=9)
@@ -239,7 +242,7 @@ def test_an_infinite_value_reaches_those_who_see_it(N):
 
 
 def test_a_nan_query_spoils_its_own_row_only():
-    for N in (3, 30):
+    for N in (3, 30, 55):
         c, k, v, gen = filled(16, 1, 60, 2, 64, [60], seed=2)
         q = torch.randn(1, N, 4, 64, generator=gen, device="cuda")
         clean = kvcache.Attention(c, n_tokens=N, heads=4)(q)
