@@ -1288,20 +1288,31 @@ template <int D, int FMT>
 int attn_launch_tc(const AttnP& P, bool general, cudaStream_t st);
 
 template <int D, int FMT>
+int attn_launch_tile(const AttnP& P, bool general, cudaStream_t st) {
+    constexpr int smem = TileCfg<D, FMT>::kSmem;
+    static PerDeviceFlag raised[2];
+    const dim3 grid(P.row_tiles * P.nsplit, P.kv_heads, P.n_seqs);
+    if (general) {
+        if (!raise_dynamic_smem(attn_tile_kernel<D, FMT, true>, smem, raised[0])) return KCB_LAUNCH_FAILURE;
+        attn_tile_kernel<D, FMT, true><<<grid, 128, smem, st>>>(P);
+    } else {
+        if (!raise_dynamic_smem(attn_tile_kernel<D, FMT, false>, smem, raised[1])) return KCB_LAUNCH_FAILURE;
+        attn_tile_kernel<D, FMT, false><<<grid, 128, smem, st>>>(P);
+    }
+    return launch_status();
+}
+template <int D, int FMT>
 int attn_launch_kernels(const AttnP& P, bool general, AttnKernel which, cudaStream_t st) {
     if (which == AttnKernel::tc) {
-        if (const int e = attn_launch_tc<D, FMT>(P, general, st); e != KCB_SUCCESS) return e;
-    } else if (which == AttnKernel::tile) {
-        constexpr int smem = TileCfg<D, FMT>::kSmem;
-        static PerDeviceFlag raised[2];
-        const dim3 grid(P.row_tiles * P.nsplit, P.kv_heads, P.n_seqs);
-        if (general) {
-            if (!raise_dynamic_smem(attn_tile_kernel<D, FMT, true>, smem, raised[0])) return KCB_LAUNCH_FAILURE;
-            attn_tile_kernel<D, FMT, true><<<grid, 128, smem, st>>>(P);
-        } else {
-            if (!raise_dynamic_smem(attn_tile_kernel<D, FMT, false>, smem, raised[1])) return KCB_LAUNCH_FAILURE;
-            attn_tile_kernel<D, FMT, false><<<grid, 128, smem, st>>>(P);
+        int e = attn_launch_tc<D, FMT>(P, general, st);
+        if (e == KCB_UNSUPPORTED_OPERATION) {  // strides that a tensor map does not take (sequences that share one cache: stride 0)
+            AttnP T = P;
+            T.row_tiles = (P.rows + QTile<D>::kRows - 1) / QTile<D>::kRows;
+            e = attn_launch_tile<D, FMT>(T, true, st);
         }
+        if (e != KCB_SUCCESS) return e;
+    } else if (which == AttnKernel::tile) {
+        if (const int e = attn_launch_tile<D, FMT>(P, general, st); e != KCB_SUCCESS) return e;
     } else {
         constexpr int smem = RowsCfg<D, FMT>::kSmem;
         static PerDeviceFlag raised[2];

@@ -4,23 +4,26 @@
 // products with a query or probability the smallest, lo * lo (2^-22), is left out.
 //
 // Three warpgroups.
-//   * Two softmax warpgroups, one query row per thread, take the 64-key tiles in turn; each has its own running maximum, sum and
-//     output, joined at the end.  Per tile one thread of the warpgroup issues the score products (queries are the A operand, resident
-//     in TMEM; keys from shared memory), every thread turns its row's 64 scores into probabilities and stores them, as hi and lo
-//     halves, over the scores in TMEM, and one thread issues the value products.  While one warpgroup computes probabilities the
-//     tensor core works for the other.
+//   * Two softmax warpgroups, one query row per thread in each: a tile of keys is cut into halves, and each warpgroup has its half of
+//     every tile, with its own running maximum, sum and output, joined at the end.  Per tile a thread reads its row's scores from
+//     TMEM, turns them into probabilities and stores those, as hi and lo halves, to TMEM, the A operand of the value products.
+//   * The rest: one warp issues all products -- scores of the next tile as soon as both warpgroups have read this one's, so that they
+//     run under the softmax -- and the others bring keys and values into rings of stages in the 128-byte-swizzled layout of the
+//     operands: fp16 rows by tensor copies that one thread issues, 4-bit rows unpacked through registers.
 //   * A tile's output starts from zero in TMEM and is added to the thread's running output in registers, in fp32: no rescaling in
-//     TMEM, and the length of the context never meets the truncation of the tensor cores' sums.  The read-back runs under the next
-//     score products.
-//   * One producer warpgroup brings key and value tiles into a ring of stages in the 128-byte-swizzled layout of the operands
-//     (cp.async for fp16 rows, registers for 4-bit rows).  It copies rows in use only (zeros behind them) and looks for values
-//     that are not finite, which would reach rows that do not see them as 0 * inf.  That is also why it is not a tensor copy.
-// TMEM (512 columns at D = 128): queries hi | lo, 64 columns of scores / probabilities and D columns of output per warpgroup.
-// Every wait is bounded: on expiry the CTA raises a flag that all roles poll, waits for its copies and products in flight, counts
-// the event, frees its TMEM and returns.
+//     TMEM, and the length of the context never meets the truncation of the tensor cores' sums.
+// TMEM (512 columns at D = 128, fp16): scores of both halves 2 * 64, probabilities 2 * 64, outputs 2 * 128.
+// Values that are not finite would reach rows that do not see them as 0 * inf, and so would what lies behind the rows in use, which
+// a tensor copy brings along.  Looking for such values costs a third of the kernel's time, so the first pass does not: where an output
+// is not finite at its end, the CTA takes a second pass that does, clears them from the tiles, and gives them to the rows that see
+// them one by one.  (4-bit rows need none: the unpacking turns scales that are not finite into zeros.)
+// Every wait is bounded: on expiry the CTA raises a flag that all roles poll, runs on without products, waits for its copies and
+// products in flight, counts the event, frees its TMEM and returns.
 #pragma once
 
 #include "kv_attention.cuh"
+
+#include <cuda.h>  // CUtensorMap and its enums; the encoder itself is looked up through the runtime (no libcuda link)
 
 namespace kcb {
 
@@ -28,28 +31,38 @@ static __device__ unsigned g_attn_timeouts = 0;
 
 template <int D, int FMT>
 struct TcCfg {
-    static constexpr int KT = 64, kRows = 128, kThreads = 384;
-    static constexpr int kPlane = KT * D * 2;                 // one fp16 tile: D / 64 atoms of 64 keys x 128 bytes
-    static constexpr int kV = (FMT == 16 ? 1 : 2) * kPlane;   // keys (hi, lo), then values (hi, lo)
-    static constexpr int kStage = 2 * kV;
-    static constexpr int kStages = (FMT == 16 ? 6 : 3) * (D == 64 ? 2 : 1) > 8 ? 8 : (FMT == 16 ? 6 : 3) * (D == 64 ? 2 : 1);
-    static constexpr int kDepth = FMT == 16 ? 3 : 0;          // tiles whose copies stay in flight behind the one being finished
-    static constexpr int kMeta = kStages * kStage;            // per stage: position and document of 64 slots, 64 bits of slots with odd values
-    static constexpr int kMetaBytes = 2 * KT * 4 + 16;
+    static constexpr int HK = FMT == 16 ? 64 : 32;             // keys of a tile per softmax warpgroup
+    static constexpr int KT = 2 * HK, kRows = 128;
+    static constexpr int kThreads = FMT == 16 ? 384 : 512, kMmaWarp = kThreads / 32 - 1, kProducers = kThreads - 256 - 32;
+    static constexpr int kPlane = KT * D * 2;                  // one fp16 tile: D / 64 atoms of KT keys x 128 bytes
+    static constexpr int kSlot = (FMT == 16 ? 1 : 2) * kPlane; // keys or values of a tile (4 bits: hi, lo)
+    static constexpr int kStages = D == 64 ? 4 : 2;            // of keys, and of values
+    static constexpr int kQHalf = kRows * D * 2;               // hi, then lo queries
+    static constexpr int kOffK = 2 * kQHalf, kOffV = kOffK + kStages * kSlot;
+    static constexpr int kMeta = kOffV + kStages * kSlot;      // per stage: KT positions, KT documents, 16 bytes free, bits of odd slots
+    static constexpr int kMetaBytes = 2 * KT * 4 + 32;
     static constexpr int kBars = kMeta + kStages * kMetaBytes;
-    static constexpr int kTile0 = kBars + 256;                // bitmap of tiles
-    static constexpr int kSmem = kTile0 + kDocBits / 8 + 1024;  // + room to align the base to 1024 bytes
-    static constexpr uint32_t kQ = 0, kS = D, kO = D + 2 * KT;  // TMEM columns
-    static constexpr int kRegsSoftmax = FMT == 16 ? 224 : 216, kRegsProducer = FMT == 16 ? 56 : 72, kRegsLaunch = 168;
-    static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsProducer <= kThreads * kRegsLaunch, "the softmax warpgroups take what the producers give up");
-    static_assert(kO + 2 * D <= 512 && 128 * D * 4 + 2048 <= kStages * kStage && kSmem <= kMaxSmem, "TMEM columns; the exchange at the end reuses the ring");
+    static constexpr int kTile0 = kBars + 256;                 // bitmap of tiles
+    static constexpr int kSmem = kTile0 + kDocBits / 8 + 1024; // + room to align the base to 1024 bytes
+    static constexpr uint32_t kS = 0, kP = KT, kO = 2 * KT;    // TMEM columns
+    static constexpr int kRegsSoftmax = FMT == 16 ? 224 : 184, kRegsProducer = FMT == 16 ? 56 : 72, kRegsLaunch = FMT == 16 ? 168 : 128;
+    static_assert(2 * 128 * kRegsSoftmax + (kThreads - 256) * kRegsProducer <= kThreads * kRegsLaunch, "the softmax warpgroups take what the producers give up");
+    static_assert(kO + 2 * D <= 512 && kMetaBytes % 16 == 0 && kSmem <= kMaxSmem && kSmem > kMaxSmem / 2, "TMEM columns; one CTA per SM");
+    static_assert(128 * D * 4 + 2048 <= 2 * kStages * kSlot, "the exchange at the end reuses the rings");
 };
 
 __device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t lbo) {  // 128-byte swizzle, 8-row groups 1024 bytes apart
     return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(lbo >> 4) << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
            (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
 }
-// D (TMEM, fp32) (+)= A (TMEM, fp16) B (shared memory, fp16)
+// D (TMEM, fp32) (+)= A B, fp16: A in shared memory or in TMEM, B in shared memory
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0)
+        : "memory");
+}
 __device__ __forceinline__ void tc_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -82,7 +95,7 @@ __device__ __forceinline__ unsigned tc_ld1(uint32_t addr) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;" : "=r"(r) : "r"(addr) : "memory");
     return r;
 }
-__device__ __forceinline__ void tc_st16(uint32_t addr, const unsigned (&r)[16]) {
+__device__ __forceinline__ void tc_st16(uint32_t addr, const unsigned* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
                  "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
                  : "memory");
@@ -90,6 +103,12 @@ __device__ __forceinline__ void tc_st16(uint32_t addr, const unsigned (&r)[16]) 
 __device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void bar_arrive(uint64_t* bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory"); }
+// Tiled 4-D tensor copy global -> this CTA's shared memory (no multicast); completion counted on `bar`.
+__device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+                 : "memory");
+}
 __device__ __forceinline__ void named_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 __device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile int* fail) {
     for (int i = 0; i < kMbarSpinLimit; ++i) {
@@ -100,35 +119,70 @@ __device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile
     return false;
 }
 
-// Capped scores: y = tanh(u) cap, u = y on entry.  The power series below 0.55 (see tanh_acc), elsewhere 1 - 2 / (e^2|u| + 1): there
+// Packed fp32 pairs (one instruction for two values, each rounded as the scalar operation).
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)), "l"(reinterpret_cast<unsigned long long&>(c)));
+    return reinterpret_cast<float2&>(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+    return reinterpret_cast<float2&>(r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+    return reinterpret_cast<float2&>(r);
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// Capped scores: y = tanh(u) cap, u = y on entry.  The power series below 0.55 (see tanh_series), elsewhere 1 - 2 / (e^2|u| + 1): there
 // the difference costs one bit.  A warp whose scores are all small against the cap, as most are, takes the series alone.
-__device__ __forceinline__ void cap_scores(float (&y)[2][32], float cap) {
+template <int N>
+__device__ __forceinline__ void cap_scores(float (&y)[N], float cap) {
     float big = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 64; ++k) big = fmaxf(big, fabsf(y[k >> 5][k & 31]));
+    for (int k = 0; k < N; ++k) big = fmaxf(big, fabsf(y[k]));
     const bool small = __all_sync(0xffffffffu, big < 0.55f);
 #pragma unroll
-    for (int k = 0; k < 64; ++k) {
-        const float u = y[k >> 5][k & 31];
-        float r = tanh_series(u);
-        if (!small && fabsf(u) >= 0.55f) r = copysignf(1.0f - __fdividef(2.0f, ex2(2.0f * kLog2e * fabsf(u)) + 1.0f), u);
-        y[k >> 5][k & 31] = r * cap;
+    for (int k = 0; k < N; k += 2) {
+        const float2 u = make_float2(y[k], y[k + 1]), w = mul2(u, u);
+        float2 r = fma2(both(-1.4558344e-3f), w, both(3.5921280e-3f));
+        r = fma2(r, w, both(-8.8632355e-3f));
+        r = fma2(r, w, both(2.1869488e-2f));
+        r = fma2(r, w, both(-5.3968254e-2f));
+        r = fma2(r, w, both(1.3333333e-1f));
+        r = fma2(r, w, both(-3.3333333e-1f));
+        r = fma2(mul2(u, w), r, u);
+        if (!small) {
+            if (fabsf(u.x) >= 0.55f) r.x = copysignf(1.0f - __fdividef(2.0f, ex2(2.0f * kLog2e * fabsf(u.x)) + 1.0f), u.x);
+            if (fabsf(u.y) >= 0.55f) r.y = copysignf(1.0f - __fdividef(2.0f, ex2(2.0f * kLog2e * fabsf(u.y)) + 1.0f), u.y);
+        }
+        r = mul2(r, both(cap));
+        y[k] = r.x, y[k + 1] = r.y;
     }
 }
 
 template <int D, int FMT, bool GEN>
-__global__ void __launch_bounds__(384, 1) attn_tc_kernel(const __grid_constant__ AttnP P) {
+__global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
+    attn_tc_kernel(const __grid_constant__ AttnP P, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
     using C = TcCfg<D, FMT>;
-    constexpr int KT = C::KT, NB = D / 32, CH = D / 8;
+    constexpr int HK = C::HK, KT = C::KT, NB = D / 32, CH = D / 8;
     extern __shared__ uint8_t sm_raw[];
     uint8_t* sm = sm_raw + ((1024u - (smem_u32(sm_raw) & 1023u)) & 1023u);
-    uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::kBars);  // [stage] tiles written
-    uint64_t* empty = full + C::kStages;                          // [stage] tiles read by the products
-    uint64_t* sfull = empty + C::kStages;                         // [warpgroup] scores complete
-    uint64_t* ofull = sfull + 2;                                  // [warpgroup] outputs complete
+    uint64_t* kfull = reinterpret_cast<uint64_t*>(sm + C::kBars);  // [stage] keys written
+    uint64_t* kempty = kfull + C::kStages;                         // [stage] keys read by the products
+    uint64_t* vfull = kempty + C::kStages;                         // [stage] values (and what stands beside them) written
+    uint64_t* vempty = vfull + C::kStages;
+    uint64_t* varrived = vempty + C::kStages;                      // [stage] fp16: values copied (the second pass waits for vfull, behind the search)
+    uint64_t* mfull = varrived + C::kStages;                       // [stage] fp16: positions and documents written
+    uint64_t* sfull = mfull + C::kStages;                          // scores of a tile complete
+    uint64_t* sread = sfull + 1;                                   // ... and read by both warpgroups
+    uint64_t* pfull = sread + 1;                                   // [warpgroup] probabilities stored, last output read
+    uint64_t* ofull = pfull + 2;                                   // [warpgroup] output of a tile complete
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ofull + 2);
     volatile int* fail = reinterpret_cast<volatile int*>(ofull + 3);
-    uint32_t* bits = reinterpret_cast<uint32_t*>(sm + C::kTile0);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wg = warp >> 2;
     const int rt = P.row_tiles - 1 - static_cast<int>(blockIdx.x) / P.nsplit, split = blockIdx.x % P.nsplit, kvh = blockIdx.y, s = blockIdx.z;
     const int row0 = rt * C::kRows;
@@ -138,397 +192,435 @@ __global__ void __launch_bounds__(384, 1) attn_tc_kernel(const __grid_constant__
     const int begin = min(n, split * chunk);
     int end = min(n, begin + chunk);
     const int tok0 = row0 / P.group, tok1 = (min(P.rows, row0 + C::kRows) - 1) / P.group;
-    const int prefix = GEN && P.prefix ? P.prefix[s] : 0;
+    const int prefix = P.prefix ? P.prefix[s] : 0;
     if (P.causal && !P.positions && !P.q_pos) end = max(begin, min(end, max(prefix, row_pos(P, s, n, tok1) + 1)));
     const int nt = (end - begin + KT - 1) / KT;
     const bool docs = GEN && P.q_doc != nullptr;
 
     if (tid == 0) {
-        for (int i = 0; i < C::kStages; ++i) mbar_init(&full[i], 128), mbar_init(&empty[i], 1);
-        for (int i = 0; i < 2; ++i) mbar_init(&sfull[i], 1), mbar_init(&ofull[i], 1);
+        for (int i = 0; i < C::kStages; ++i) {
+            mbar_init(&kfull[i], FMT == 16 ? 1 : C::kProducers), mbar_init(&kempty[i], 1), mbar_init(&vfull[i], C::kProducers), mbar_init(&vempty[i], 1);
+            mbar_init(&varrived[i], 1), mbar_init(&mfull[i], 64);
+        }
+        mbar_init(sfull, 1), mbar_init(sread, 256);
+        for (int i = 0; i < 2; ++i) mbar_init(&pfull[i], 128), mbar_init(&ofull[i], 1);
         *fail = 0;
         mbar_init_fence();
     }
-    if (warp == 8) {
+    if (warp == C::kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    const DocTiles<KT> doc_tiles{bits, nt};
-    if (docs) doc_tiles.clear(tid, C::kThreads);
+    const DocTiles<KT> doc_tiles{reinterpret_cast<uint32_t*>(sm + C::kTile0), nt};
+    if (docs) {
+        doc_tiles.clear(tid, C::kThreads);
+        __syncthreads();
+        doc_tiles.find(P, s, tok0, tok1, begin, end, warp, C::kThreads / 32, lane);
+    }
+    auto next = [&](int i) { return docs ? doc_tiles.next(i) : i + 1; };  // the tile behind tile i that is wanted
+    auto swz = [&](int rows, int r, int ch) { return (ch >> 3) * (rows * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4); };
+
+    float ysc = 0.0f;
+    if (wg < 2) {  // the rows' queries: warpgroup 0 stores the hi halves, warpgroup 1 the lo halves
+        const int r = tid & 127, row = row0 + r;
+        const bool valid = row < P.rows;
+        const int token = (valid ? row : 0) / P.group, head = kvh * P.group + (valid ? row : 0) % P.group;
+        const float4* qp = reinterpret_cast<const float4*>(P.q + static_cast<size_t>(s) * P.q_seq + static_cast<size_t>(token) * P.q_token + static_cast<size_t>(head) * P.q_head);
+        const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float amax = 0.0f;
+#pragma unroll 8
+        for (int i = 0; i < D / 4; ++i) {
+            const float4 f = valid ? qp[i] : zero;
+            amax = fmaxf(fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y))), fmaxf(fabsf(f.z), fabsf(f.w)));
+        }
+        float up, down;
+        row_scale(amax, up, down);
+        ysc = P.sc * down;
+#pragma unroll 4
+        for (int ch = 0; ch < CH; ++ch) {
+            const float4 a = valid ? qp[2 * ch] : zero, b = valid ? qp[2 * ch + 1] : zero;
+            uint4 hi, lo;
+            split2(a.x * up, a.y * up, hi.x, lo.x);
+            split2(a.z * up, a.w * up, hi.y, lo.y);
+            split2(b.x * up, b.y * up, hi.z, lo.z);
+            split2(b.z * up, b.w * up, hi.w, lo.w);
+            *reinterpret_cast<uint4*>(sm + wg * C::kQHalf + swz(C::kRows, r, ch)) = wg ? lo : hi;
+        }
+        fence_async_shared();
+    }
     tc_before_sync();
     __syncthreads();
     tc_after_sync();
     const uint32_t tmem = *tmem_slot;
-    if (docs) doc_tiles.find(P, s, tok0, tok1, begin, end, warp, C::kThreads / 32, lane);
-    auto next = [&](int i) { return docs ? doc_tiles.next(i) : i + 1; };  // the tile behind tile i that is wanted
+    // (after an expired wait every loop below runs on, without products, so that every barrier finds its arrivals)
 
-    if (wg == 2) {
-        // ---- producers ----------------------------------------------------------------------------------------------------
+    if (wg >= 2) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsProducer));
-        if (docs) __syncthreads();
-        __syncthreads();  // (the queries)
-        const int ptid = tid - 256;
-        const bool hides = GEN || P.causal;
-        auto swz = [&](int r, int ch) { return (ch >> 3) * (KT * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4); };
-        auto copy = [&](int tile, int stage) {  // fp16: start the copies
-            const uint32_t dst = smem_u32(sm) + stage * C::kStage;
-            const int t0 = begin + tile * KT;
-            const __half* kb = reinterpret_cast<const __half*>(P.k) + static_cast<size_t>(s) * P.k_seq + static_cast<size_t>(kvh) * P.k_head;
-            const __half* vb = reinterpret_cast<const __half*>(P.v) + static_cast<size_t>(s) * P.v_seq + static_cast<size_t>(kvh) * P.v_head;
+        if (warp == C::kMmaWarp) {
+            // ---- products ----------------------------------------------------------------------------------------------------
+            int i = 0;  // tiles so far, over both passes: stages and parities go by it
+            for (bool careful = false;; careful = true) {
+                const int i0 = i;
+                if (lane == 0) {
+                    const uint32_t base = smem_u32(sm);
+                    constexpr uint32_t kIdescS = (1u << 4) | (static_cast<uint32_t>(KT >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
+                    constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
+                    uint64_t* vready = FMT == 16 && !careful ? varrived : vfull;
+                    auto scores = [&](int j) {  // (hi + lo) keys^T, both halves of the tile
+                        const int st = j % C::kStages;
+                        tc_wait(&kfull[st], (j / C::kStages) & 1, fail);
+                        tc_after_sync();
+                        if (*fail) return;
+                        const uint32_t kb = base + C::kOffK + st * C::kSlot;
 #pragma unroll
-            for (int i = 0; i < KT * CH / 128; ++i) {
-                const int x = i * 128 + ptid, r = x / CH, ch = x % CH;
-                const bool ok = t0 + r < end;
-                const size_t t = ok ? t0 + r : 0;
-                cp16(dst + swz(r, ch), kb + t * P.k_row + ch * 8, ok);
-                cp16(dst + C::kV + swz(r, ch), vb + t * P.v_row + ch * 8, ok);
-            }
-        };
-        auto finish = [&](int tile, int stage) {
-            const int t0 = begin + tile * KT;
-            uint8_t* st = sm + stage * C::kStage;
-            int* meta = reinterpret_cast<int*>(sm + C::kMeta + stage * C::kMetaBytes);
-            if (GEN && ptid < KT) {
-                const KeyInfo key = key_info(P, s, kvh, t0 + ptid, end);
-                meta[ptid] = key.pos, meta[KT + ptid] = key.doc;
-            }
-            if (FMT == 16) {
-                if (hides) {
-                    unsigned* odd = reinterpret_cast<unsigned*>(meta + 2 * KT);
-                    bool any = false;
-#pragma unroll
-                    for (int i = 0; i < KT * CH / 128; ++i) {  // the chunks this thread copied itself
-                        const int x = i * 128 + ptid;
-                        any = any || not_finite(*reinterpret_cast<const uint4*>(st + C::kV + swz(x / CH, x % CH)));
-                    }
-                    if (any) {
-#pragma unroll 1
-                        for (int i = 0; i < KT * CH / 128; ++i) {
-                            const int x = i * 128 + ptid;
-                            uint8_t* at = st + C::kV + swz(x / CH, x % CH);
-                            if (!not_finite(*reinterpret_cast<const uint4*>(at))) continue;
-                            zero_not_finite(at);
-                            atomicOr(&odd[(x / CH) >> 5], 1u << ((x / CH) & 31));
+                        for (int k = 0; k < D / 16; ++k) {
+                            const uint64_t qh = tc_desc(base + (k >> 2) * (C::kRows * 128) + (k & 3) * 32, 0), ql = qh + (C::kQHalf >> 4);
+                            const uint64_t kd = tc_desc(kb + (k >> 2) * (KT * 128) + (k & 3) * 32, 0);
+                            tc_mma_ss(tmem + C::kS, qh, kd, kIdescS, k > 0);
+                            tc_mma_ss(tmem + C::kS, ql, kd, kIdescS, 1);
+                            if (FMT != 16) tc_mma_ss(tmem + C::kS, qh, kd + (C::kPlane >> 4), kIdescS, 1);
                         }
+                        tc_commit(sfull);
+                        tc_commit(&kempty[st]);
+                    };
+                    int tile = next(-1);
+                    if (tile < nt) scores(i);
+                    while (tile < nt) {
+                        tile = next(tile);
+                        tc_wait(sread, i & 1, fail);
+                        if (tile < nt) scores(i + 1);
+                        const int st = i % C::kStages;
+                        const uint32_t vb = base + C::kOffV + st * C::kSlot;
+                        tc_wait(&vready[st], ((i - (careful ? i0 : 0)) / C::kStages) & 1, fail);  // (vfull completes in the second pass alone)
+#pragma unroll
+                        for (int w = 0; w < 2; ++w) {
+                            tc_wait(&pfull[w], i & 1, fail);
+                            tc_after_sync();
+                            if (*fail) continue;
+#pragma unroll
+                            for (int k = 0; k < HK / 16; ++k) {
+                                const uint32_t ph = tmem + C::kP + w * HK + k * 8, pl = ph + HK / 2, od = tmem + C::kO + w * D;
+                                const uint64_t vd = tc_desc(vb + (w * HK + k * 16) * 128, KT * 128);
+                                tc_mma(od, ph, vd, kIdescO, k > 0);
+                                tc_mma(od, pl, vd, kIdescO, 1);
+                                if (FMT != 16) tc_mma(od, ph, vd + (C::kPlane >> 4), kIdescO, 1);
+                            }
+                            tc_commit(&ofull[w]);
+                        }
+                        if (!*fail) tc_commit(&vempty[st]);
+                        ++i;
                     }
                 }
-            } else {
-                // 4 bits: a thread takes a quarter of the key row's and of the value row's groups; two threads to a row
-                const uint8_t* kb = P.k + static_cast<size_t>(s) * P.seq_bytes;
-                const uint8_t* vb = P.v + static_cast<size_t>(s) * P.seq_bytes;
-#pragma unroll
-                for (int plane = 0; plane < 2; ++plane) {
-                    const int r = ptid >> 1, half = ptid & 1;
+                __syncwarp();
+                if (FMT != 16 || !__syncthreads_or(0) || careful) break;
+            }
+        } else {
+            // ---- producers ---------------------------------------------------------------------------------------------------
+            const int ptid = tid - 256;
+            auto unpack = [&](const uint8_t* src, bool value, uint8_t* dst, int t0) {  // 4 bits: values as hi and lo tiles
+                const uint8_t* b0 = src + static_cast<size_t>(s) * P.seq_bytes;
+                // an item is group c of a row: the pieces (b, c) of 8 channels of every block b (values: groups 2 c and 2 c + 1)
+#pragma unroll 1
+                for (int x = ptid; x < KT * 4; x += C::kProducers) {
+                    const int r = x >> 2, c = x & 3;
                     const bool ok = t0 + r < end;
                     const size_t at = static_cast<size_t>(kvh) * P.cap + (ok ? t0 + r : 0);
-                    const uint8_t* rowp = (plane ? vb : kb) + at * (D / 2);
-                    const unsigned* par = reinterpret_cast<const unsigned*>((plane ? vb : kb) + P.par_off + at * (4 * NB));
-                    uint8_t* hi_t = st + (plane ? C::kV : 0);
-                    float d[NB], m[NB];
+                    const uint8_t* rowp = b0 + at * (D / 2);
+                    const unsigned* par = reinterpret_cast<const unsigned*>(b0 + P.par_off + at * (4 * NB));
+                    unsigned pw[NB], v[NB];
+                    if constexpr (NB == 4) {
+                        const uint4 t = *reinterpret_cast<const uint4*>(rowp + c * 16), q = *reinterpret_cast<const uint4*>(par);
+                        v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
+                        pw[0] = q.x, pw[1] = q.y, pw[2] = q.z, pw[3] = q.w;
+                    } else {
+                        const uint2 t = *reinterpret_cast<const uint2*>(rowp + c * 8), q = *reinterpret_cast<const uint2*>(par);
+                        v[0] = t.x, v[1] = t.y;
+                        pw[0] = q.x, pw[1] = q.y;
+                    }
 #pragma unroll
                     for (int b = 0; b < NB; ++b) {
-                        unsigned w = ok ? par[b] : 0u;
-                        if ((w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u) w = 0u;  // (a hidden slot's scales may be anything)
-                        d[b] = half_bits_to_float(w & 0xFFFFu), m[b] = half_bits_to_float(w >> 16);
-                    }
-                    // 16-byte pieces of 8 channels: piece 4 b + c of a row; a key row's group c holds the pieces (b, c)
-                    // whole, a value row's groups 2 c and 2 c + 1 half of each
+                        // a row behind those in use is zeros, and a hidden slot's scales may be anything
+                        if (!ok || not_finite2(pw[b])) pw[b] = 0u;
+                        const unsigned w = value ? __byte_perm(v[b / 2], v[NB / 2 + b / 2], b & 1 ? 0x7632 : 0x5410) : v[b];
+                        const float2 dm = __half22float2(*reinterpret_cast<__half2*>(&pw[b]));
+                        // codes about their middle, 2^23 + code less 2^23 + 8: no integer conversion
+                        const float2 d = both(dm.x), mid = both(fmaf(8.0f, dm.x, dm.y));
+                        unsigned hi[4], lo[4];
 #pragma unroll
-                    for (int cc = 0; cc < 2; ++cc) {
-                        const int c = half * 2 + cc;
-                        unsigned v[NB], w[NB];  // the piece's 4 NB bytes, and 8 codes per block
-                        if (ok) {
-                            if constexpr (NB == 4) {
-                                const uint4 t = *reinterpret_cast<const uint4*>(rowp + c * 16);
-                                v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
-                            } else {
-                                const uint2 t = *reinterpret_cast<const uint2*>(rowp + c * 8);
-                                v[0] = t.x, v[1] = t.y;
-                            }
-                        } else {
-#pragma unroll
-                            for (int b = 0; b < NB; ++b) v[b] = 0u;
+                        for (int k = 0; k < 4; ++k) {
+                            const float2 code = add2(make_float2(__uint_as_float(0x4B000000u | (w >> (8 * k) & 15u)), __uint_as_float(0x4B000000u | (w >> (8 * k + 4) & 15u))), both(-8388616.0f));
+                            const float2 x2 = fma2(d, code, mid);
+                            const __half2 h = __floats2half2_rn(fminf(x2.x, 65504.0f), fminf(x2.y, 65504.0f));  // the rest of a larger value goes to lo
+                            const float2 f = __half22float2(h);
+                            hi[k] = h2_bits(h), lo[k] = h2_bits(__floats2half2_rn(x2.x - f.x, x2.y - f.y));
                         }
-#pragma unroll
-                        for (int b = 0; b < NB; ++b) w[b] = plane == 0 ? v[b] : __byte_perm(v[b / 2], v[NB / 2 + b / 2], b & 1 ? 0x7632 : 0x5410);
-#pragma unroll
-                        for (int b = 0; b < NB; ++b) {
-                            uint4 hi, lo;
-                            unsigned* hp = &hi.x;
-                            unsigned* lp = &lo.x;
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const float x = fmaf(d[b], static_cast<float>(w[b] >> (8 * k) & 15u), m[b]), y = fmaf(d[b], static_cast<float>(w[b] >> (8 * k + 4) & 15u), m[b]);
-                                const __half2 h = __floats2half2_rn(fminf(x, 65504.0f), fminf(y, 65504.0f));  // the rest of a larger value goes to lo
-                                const float2 f = __half22float2(h);
-                                hp[k] = h2_bits(h), lp[k] = h2_bits(__floats2half2_rn(x - f.x, y - f.y));
-                            }
-                            const int o = swz(r, 4 * b + c);
-                            *reinterpret_cast<uint4*>(hi_t + o) = hi;
-                            *reinterpret_cast<uint4*>(hi_t + C::kPlane + o) = lo;
-                        }
+                        uint8_t* o = dst + swz(KT, r, 4 * b + c);
+                        *reinterpret_cast<uint4*>(o) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4*>(o + C::kPlane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                     }
                 }
+            };
+            auto beside = [&](int t0, int st, int first, int threads) {  // positions and documents of a tile's slots
+                int* meta = reinterpret_cast<int*>(sm + C::kMeta + st * C::kMetaBytes);
+                for (int k = first; k < KT; k += threads) {
+                    const KeyInfo key = key_info(P, s, kvh, t0 + k, end);
+                    meta[k] = key.pos, meta[KT + k] = key.doc;
+                }
+            };
+            const bool beside_wanted = GEN && (P.positions || P.k_doc);
+            int i = 0;
+            if constexpr (FMT != 16) {
+                for (int tile = next(-1); tile < nt; tile = next(tile), ++i) {
+                    const int st = i % C::kStages, ph = (i / C::kStages - 1) & 1, t0 = begin + tile * KT;
+                    if (i >= C::kStages) tc_wait(&kempty[st], ph, fail);
+                    unpack(P.k, false, sm + C::kOffK + st * C::kSlot, t0);
+                    fence_async_shared();
+                    bar_arrive(&kfull[st]);
+                    if (i >= C::kStages) tc_wait(&vempty[st], ph, fail);
+                    unpack(P.v, true, sm + C::kOffV + st * C::kSlot, t0);
+                    if (beside_wanted) beside(t0, st, ptid, C::kProducers);
+                    fence_async_shared();
+                    bar_arrive(&vfull[st]);
+                }
+            } else {
+                for (bool careful = false;; careful = true) {
+                    const int i0 = i;
+                    for (int tile = next(-1); tile < nt; tile = next(tile), ++i) {
+                        const int st = i % C::kStages, ph = (i / C::kStages - 1) & 1, t0 = begin + tile * KT;
+                        uint8_t* vt = sm + C::kOffV + st * C::kSlot;
+                        if (warp == 8 && lane == 0) {
+                            if (i >= C::kStages) tc_wait(&kempty[st], ph, fail);
+                            mbar_expect_tx(&kfull[st], C::kSlot);
+#pragma unroll
+                            for (int h = 0; h < D / 64; ++h) tma_4d(smem_u32(sm) + C::kOffK + st * C::kSlot + h * (KT * 128), &map_k, h * 64, kvh, t0, s, &kfull[st]);
+                            if (i >= C::kStages) tc_wait(&vempty[st], ph, fail);
+                            mbar_expect_tx(&varrived[st], C::kSlot);
+#pragma unroll
+                            for (int h = 0; h < D / 64; ++h) tma_4d(smem_u32(vt) + h * (KT * 128), &map_v, h * 64, kvh, t0, s, &varrived[st]);
+                        }
+                        if (warp != 8 && beside_wanted) {
+                            if (i >= C::kStages) tc_wait(&vempty[st], ph, fail);
+                            beside(t0, st, ptid - 32, 64);
+                            bar_arrive(&mfull[st]);
+                        }
+                        if (careful) {
+                            __syncwarp();
+                            unsigned* odd = reinterpret_cast<unsigned*>(sm + C::kMeta + st * C::kMetaBytes + 2 * KT * 4 + 16);
+                            tc_wait(&varrived[st], (i / C::kStages) & 1, fail);
+                            if (ptid < KT / 32) odd[ptid] = 0u;
+                            named_sync(3, C::kProducers);  // nobody sets a bit before they are cleared
+#pragma unroll 1
+                            for (int x = ptid; x < KT * CH; x += C::kProducers) {
+                                uint8_t* at = vt + swz(KT, x / CH, x % CH);
+                                if (!not_finite(*reinterpret_cast<const uint4*>(at))) continue;
+                                zero_not_finite(at);
+                                atomicOr(&odd[(x / CH) >> 5], 1u << ((x / CH) & 31));
+                            }
+                            fence_async_shared();
+                            bar_arrive(&vfull[st]);
+                        }
+                    }
+                    __syncwarp();
+                    if (!__syncthreads_or(0) || careful) break;
+                }
             }
-            fence_async_shared();
-            bar_arrive(&full[stage]);
-        };
-        // tile number i (in order of use) goes to stage i % kStages
-        int put = 0, done = 0, tile = next(-1), ready = tile;
-        while (done < put || tile < nt) {
-            if (tile < nt && put - done <= C::kDepth) {
-                const int stage = put % C::kStages;
-                if (put >= C::kStages) tc_wait(&empty[stage], (put / C::kStages - 1) & 1, fail);
-                if (ptid < 2) reinterpret_cast<unsigned*>(sm + C::kMeta + stage * C::kMetaBytes + 2 * KT * 4)[ptid] = 0u;
-                named_sync(3, 128);  // the odd-value bits are cleared before anybody sets one
-                if (FMT == 16) copy(tile, stage);
-                cp_commit();
-                tile = next(tile), ++put;
-                if (put - done <= C::kDepth && tile < nt) continue;
-            }
-            if (tile < nt) cp_wait<C::kDepth>();
-            else cp_wait<0>();
-            finish(ready, done % C::kStages);
-            ready = next(ready), ++done;
         }
-        cp_wait<0>();
     } else {
         // ---- softmax -------------------------------------------------------------------------------------------------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsSoftmax));
-        if (docs) __syncthreads();
         const int r = tid & 127, row = row0 + r;
-        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem + C::kS + wg * KT, to = tmem + C::kO + wg * D;
         const bool valid = row < P.rows;
-        float ysc;
-        {  // the row's query: warpgroup 0 stores the hi halves, warpgroup 1 the lo halves
-            const int token = (valid ? row : 0) / P.group, head = kvh * P.group + (valid ? row : 0) % P.group;
-            const float4* qp = reinterpret_cast<const float4*>(P.q + static_cast<size_t>(s) * P.q_seq + static_cast<size_t>(token) * P.q_token + static_cast<size_t>(head) * P.q_head);
-            float amax = 0.0f;
-#pragma unroll 8
-            for (int i = 0; i < D / 4; ++i) {
-                const float4 f = valid ? qp[i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                amax = fmaxf(fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y))), fmaxf(fabsf(f.z), fabsf(f.w)));
-            }
-            float up, down;
-            row_scale(amax, up, down);
-            ysc = P.sc * down;
-#pragma unroll
-            for (int i = 0; i < D / 32; ++i) {
-                unsigned out[16];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const float4 f = valid ? qp[i * 8 + k] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    unsigned h0, l0, h1, l1;
-                    split2(f.x * up, f.y * up, h0, l0);
-                    split2(f.z * up, f.w * up, h1, l1);
-                    out[2 * k] = wg ? l0 : h0, out[2 * k + 1] = wg ? l1 : h1;
-                }
-                tc_st16(tmem + lanes + C::kQ + wg * (D / 2) + i * 16, out);
-            }
-            tc_st_wait();
-        }
-        tc_before_sync();
-        __syncthreads();
-        tc_after_sync();
-
-        const uint32_t base = smem_u32(sm);
-        constexpr uint32_t kIdescS = (1u << 4) | (static_cast<uint32_t>(KT >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
-        constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
-        auto issue_scores = [&](int i) {  // tile number i: scores = (hi + lo) keys^T
-            const uint32_t st = base + (i % C::kStages) * C::kStage;
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-                const uint32_t at = st + (k >> 2) * (KT * 128) + (k & 3) * 32;
-                const uint32_t qh = tmem + C::kQ + k * 8, ql = qh + D / 2;
-                tc_mma(ts, qh, tc_desc(at, 0), kIdescS, k > 0);
-                tc_mma(ts, ql, tc_desc(at, 0), kIdescS, 1);
-                if (FMT != 16) tc_mma(ts, qh, tc_desc(at + C::kPlane, 0), kIdescS, 1);
-            }
-            tc_commit(&sfull[wg]);
-        };
-        auto issue_values = [&](int i) {
-            const uint32_t st = base + (i % C::kStages) * C::kStage + C::kV;
-#pragma unroll
-            for (int k = 0; k < KT / 16; ++k) {
-                const uint32_t at = st + k * 2048;
-                const uint32_t ph = ts + k * 8, pl = ph + KT / 2;
-                tc_mma(to, ph, tc_desc(at, KT * 128), kIdescO, k > 0);
-                tc_mma(to, pl, tc_desc(at, KT * 128), kIdescO, 1);
-                if (FMT != 16) tc_mma(to, ph, tc_desc(at + C::kPlane, KT * 128), kIdescO, 1);
-            }
-            tc_commit(&ofull[wg]);
-            tc_commit(&empty[i % C::kStages]);
-        };
-        RowInfo ri;
-        int limit = n;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + C::kS + wg * HK + lanes, tp = tmem + C::kP + wg * HK + lanes, to = tmem + C::kO + wg * D + lanes;
+        RowInfo ri{};
         if (GEN) ri = row_info(P, s, kvh, n, row);
-        else if (P.causal) limit = valid ? min(n, row_pos(P, s, n, row / P.group) + 1) : 0;
-        limit = min(limit, end);
+        // slots from `limit` on are hidden by the end of the range, or (slot = position) by causality
+        int limit = valid ? end : 0;
+        if (P.causal && valid && !(GEN && P.positions)) limit = min(end, max(prefix, row_pos(P, s, n, row / P.group) + 1));
 
-        float o[D], m = -INFINITY, l = 0.0f;
+        float2 o[D / 2];
+        float m, l, al;
+        auto drain = [&]() {  // o = o al + the last tile's output
 #pragma unroll
-        for (int i = 0; i < D; ++i) o[i] = 0.0f;
-        const bool elected = (tid & 127) == 0;
-        // tile numbers wg, wg + 2, ...: `tile` is the one of number i
-        int tile = next(-1);
-        if (wg) tile = next(tile);
-        if (tile < nt && elected) {
-            if (tc_wait(&full[wg], 0, fail)) issue_scores(wg);
-        }
-        // (after an expired wait the loops run on, without products, so that every barrier finds its threads)
-        uint32_t round = 0;
-        for (int i = wg; tile < nt; i += 2, ++round) {
-            const int stage = i % C::kStages;
-            tc_wait(&sfull[wg], round & 1, fail);
-            tc_wait(&full[stage], (i / C::kStages) & 1, fail);  // (long complete: makes what the producers wrote beside the tiles visible)
+            for (int h = 0; h < D / 32; ++h) {
+                float v[32];
+                tc_ld32(to + h * 32, v);
+                tc_ld_wait(v);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) o[h * 16 + k] = fma2(o[h * 16 + k], both(al), make_float2(v[2 * k], v[2 * k + 1]));
+            }
+        };
+        int i = 0;  // tiles so far, over both passes
+        for (bool careful = false;; careful = true) {
+        const int i0 = i;
+        m = -INFINITY, l = 0.0f, al = 1.0f;
+#pragma unroll
+        for (int k = 0; k < D / 2; ++k) o[k] = make_float2(0.0f, 0.0f);
+        for (int tile = next(-1); tile < nt; tile = next(tile), ++i) {
+            const int t0 = begin + tile * KT + wg * HK;  // this warpgroup's first slot
+            const int st = i % C::kStages;
+            const int* meta = reinterpret_cast<const int*>(sm + C::kMeta + st * C::kMetaBytes) + wg * HK;
+            tc_wait(sfull, i & 1, fail);
             __syncwarp();
             tc_after_sync();
-            float y[2][32];
-            tc_ld32(ts + lanes, y[0]);
-            tc_ld32(ts + lanes + 32, y[1]);
-            tc_ld_wait(y[0]);
-            tc_ld_wait(y[1]);
-            const int t0 = begin + tile * KT;
-            if (!GEN) {
+            float y[HK];
+            tc_ld32(ts, reinterpret_cast<float(&)[32]>(y[0]));
+            if (HK == 64) tc_ld32(ts + 32, reinterpret_cast<float(&)[32]>(y[HK - 32]));
+            tc_ld_wait(reinterpret_cast<float(&)[32]>(y[0]));
+            if (HK == 64) tc_ld_wait(reinterpret_cast<float(&)[32]>(y[HK - 32]));
+            tc_before_sync();
+            bar_arrive(sread);
 #pragma unroll
-                for (int k = 0; k < KT; ++k) y[k >> 5][k & 31] *= ysc;
-                if (!__all_sync(0xffffffffu, t0 + KT <= limit)) {
-#pragma unroll
-                    for (int k = 0; k < KT; ++k)
-                        if (t0 + k >= limit) y[k >> 5][k & 31] = -INFINITY;
-                }
-            } else {
-                const int* meta = reinterpret_cast<const int*>(sm + C::kMeta + stage * C::kMetaBytes);
-#pragma unroll
-                for (int k = 0; k < KT; ++k) y[k >> 5][k & 31] *= ysc;
+            for (int k = 0; k < HK; k += 2) {
+                const float2 t = mul2(make_float2(y[k], y[k + 1]), both(ysc));
+                y[k] = t.x, y[k + 1] = t.y;
+            }
+            if (GEN) {
                 if (P.cap_out != 0.0f) cap_scores(y, P.cap_out);
+                if (P.positions || P.k_doc) tc_wait(FMT == 16 ? &mfull[st] : &vfull[st], (i / C::kStages) & 1, fail);
                 if (P.mask) {
                     const unsigned short* mp = ri.mask + t0;
-                    const bool wide = ((reinterpret_cast<uintptr_t>(mp) & 15) == 0) && t0 + KT <= end;
+                    const bool wide = ((reinterpret_cast<uintptr_t>(mp) & 15) == 0) && t0 + HK <= end;
 #pragma unroll
-                    for (int k8 = 0; k8 < KT / 8; ++k8) {
-                        unsigned short h[8];
+                    for (int k8 = 0; k8 < HK / 8; ++k8) {
+                        unsigned w[4];
                         if (wide) {
-                            *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(mp + 8 * k8);
+                            const uint4 t = *reinterpret_cast<const uint4*>(mp + 8 * k8);
+                            w[0] = t.x, w[1] = t.y, w[2] = t.z, w[3] = t.w;
                         } else {
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) h[k] = t0 + 8 * k8 + k < end ? mp[8 * k8 + k] : 0xFC00u;
+                            for (int k = 0; k < 4; ++k) {
+                                const int t = t0 + 8 * k8 + 2 * k;
+                                w[k] = (t < end ? mp[8 * k8 + 2 * k] : 0xFC00u) | (static_cast<unsigned>(t + 1 < end ? mp[8 * k8 + 2 * k + 1] : 0xFC00u) << 16);
+                            }
                         }
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
-                            float& v = y[k8 >> 2][(k8 & 3) * 8 + k];
-                            v = h[k] == 0xFC00u ? -INFINITY : fmaf(ri.slope, half_bits_to_float(h[k]), v);
+                            float& v = y[k8 * 8 + k];
+                            const unsigned h = w[k >> 1] >> (16 * (k & 1)) & 0xFFFFu;
+                            v = h == 0xFC00u ? -INFINITY : fmaf(ri.slope, half_bits_to_float(h), v);
                         }
                     }
                 } else if (P.bias_step != 0.0f) {
                     const float qp = static_cast<float>(ri.pos);
+                    if (P.positions) {
 #pragma unroll
-                    for (int k = 0; k < KT; ++k) y[k >> 5][k & 31] -= ri.slope * fabsf(qp - static_cast<float>(meta[k]));
+                        for (int k = 0; k < HK; ++k) y[k] -= ri.slope * fabsf(qp - static_cast<float>(meta[k]));
+                    } else {
+                        const float far = static_cast<float>(ri.pos) - static_cast<float>(t0);
+#pragma unroll
+                        for (int k = 0; k < HK; ++k) y[k] -= ri.slope * fabsf(far - static_cast<float>(k));
+                    }
                 }
-                unsigned see[2] = {valid ? 0xffffffffu : 0u, valid ? 0xffffffffu : 0u};
-                if (t0 + KT > end) {
-                    const int in = end - t0;  // 1 .. 63
-                    see[0] &= in >= 32 ? 0xffffffffu : (1u << in) - 1u;
-                    see[1] &= in <= 32 ? 0u : (1u << (in - 32)) - 1u;
-                }
-                if (P.causal && (P.positions || P.q_pos || !__all_sync(0xffffffffu, t0 + KT - 1 <= ri.pos || t0 + KT <= prefix))) {
+                if (P.causal && P.positions) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        unsigned w = 0;
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            const int kp = meta[h * 32 + k];
-                            w |= static_cast<unsigned>(kp <= ri.pos || kp < prefix) << k;
-                        }
-                        see[h] &= w;
+                    for (int k = 0; k < HK; k += 4) {
+                        const int4 kp = *reinterpret_cast<const int4*>(meta + k);
+                        if (kp.x > ri.pos && kp.x >= prefix) y[k] = -INFINITY;
+                        if (kp.y > ri.pos && kp.y >= prefix) y[k + 1] = -INFINITY;
+                        if (kp.z > ri.pos && kp.z >= prefix) y[k + 2] = -INFINITY;
+                        if (kp.w > ri.pos && kp.w >= prefix) y[k + 3] = -INFINITY;
                     }
                 }
                 if (docs) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        unsigned w = 0;
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) w |= static_cast<unsigned>(meta[KT + h * 32 + k] == ri.doc) << k;
-                        see[h] &= w;
+                    for (int k = 0; k < HK; k += 4) {
+                        const int4 kd = *reinterpret_cast<const int4*>(meta + KT + k);
+                        if (kd.x != ri.doc) y[k] = -INFINITY;
+                        if (kd.y != ri.doc) y[k + 1] = -INFINITY;
+                        if (kd.z != ri.doc) y[k + 2] = -INFINITY;
+                        if (kd.w != ri.doc) y[k + 3] = -INFINITY;
                     }
                 }
-                if (!__all_sync(0xffffffffu, (see[0] & see[1]) == 0xffffffffu)) {
+            }
+            if (!__all_sync(0xffffffffu, t0 + HK <= limit)) {
 #pragma unroll
-                    for (int k = 0; k < KT; ++k)
-                        if (!(see[k >> 5] >> (k & 31) & 1u)) y[k >> 5][k & 31] = -INFINITY;
-                }
+                for (int k = 0; k < HK; ++k)
+                    if (t0 + k >= limit) y[k] = -INFINITY;
             }
             float mx = m;
 #pragma unroll
-            for (int k = 0; k < KT; k += 2) mx = fmaxf(mx, fmaxf(y[k >> 5][k & 31], y[k >> 5][(k & 31) + 1]));
-            float al = mx > m ? ex2(m - mx) : 1.0f;
+            for (int k = 0; k < HK; k += 2) mx = fmaxf(mx, fmaxf(y[k], y[k + 1]));
+            const float al1 = mx > m ? ex2(m - mx) : 1.0f;
             m = mx;
-            const float ref = m == -INFINITY ? 0.0f : m - kPShift;
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            const float2 ref = both(m == -INFINITY ? 0.0f : kPShift - m);
+            float2 sum = make_float2(0.0f, 0.0f), sum1 = sum;
+            // the last tile's value products have read their probabilities: this tile's may take the place
+            if (i > i0) {
+                tc_wait(&ofull[wg], (i - 1) & 1, fail);
+                __syncwarp();
+                tc_after_sync();
+            }
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < HK / 32; ++h) {
                 unsigned hi[16], lo[16];
 #pragma unroll
-                for (int k = 0; k < 32; k += 2) {
-                    y[h][k] = ex2(y[h][k] - ref), y[h][k + 1] = ex2(y[h][k + 1] - ref);
-                    sum[k & 2] += y[h][k], sum[(k & 2) + 1] += y[h][k + 1];
-                    split2(y[h][k], y[h][k + 1], hi[k / 2], lo[k / 2]);
+                for (int k = 0; k < 16; ++k) {
+                    const float2 e = add2(make_float2(y[h * 32 + 2 * k], y[h * 32 + 2 * k + 1]), ref);
+                    const float2 p = make_float2(ex2(e.x), ex2(e.y));
+                    if (k & 1) sum1 = add2(sum1, p);
+                    else sum = add2(sum, p);
+                    const __half2 hh = __floats2half2_rn(p.x, p.y);
+                    const float2 f = __half22float2(hh), d = add2(p, make_float2(-f.x, -f.y));
+                    hi[k] = h2_bits(hh), lo[k] = h2_bits(__floats2half2_rn(d.x, d.y));
                 }
-                tc_st16(ts + lanes + h * 16, hi);
-                tc_st16(ts + lanes + KT / 2 + h * 16, lo);
+                tc_st16(tp + h * 16, hi);
+                tc_st16(tp + HK / 2 + h * 16, lo);
             }
-            l = fmaf(l, al, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+            sum = add2(sum, sum1);
+            l = fmaf(l, al1, sum.x + sum.y);
+            if (i > i0) drain();
+            al = al1;
             tc_st_wait();
-            if (FMT == 16) {  // rare: values of this tile that are not finite go to the rows that see them one by one
-                const unsigned* odd = reinterpret_cast<const unsigned*>(sm + C::kMeta + stage * C::kMetaBytes + 2 * KT * 4);
-                const unsigned w0 = odd[0], w1 = odd[1];
-                if (w0 | w1) {
-                    al = fmaxf(al, 1e-30f);  // an infinity added now stays one when the output is rescaled below
+            if (FMT == 16 && careful) {  // values of this tile that are not finite go to the rows that see them one by one
+                tc_wait(&vfull[st], ((i - i0) / C::kStages) & 1, fail);
+                const unsigned* odd = reinterpret_cast<const unsigned*>(sm + C::kMeta + st * C::kMetaBytes + 2 * KT * 4 + 16) + wg * (HK / 32);
+                unsigned any = 0;
+#pragma unroll
+                for (int h = 0; h < HK / 32; ++h) any |= odd[h];
+                __syncwarp();
+                if (any) {
+                    al = fmaxf(al, 1e-30f);  // an infinity added now stays one when the output is rescaled
 #pragma unroll 1
-                    for (int k = 0; k < KT; ++k) {
-                        if (!((k < 32 ? w0 >> k : w1 >> (k - 32)) & 1u)) continue;
+                    for (int k = 0; k < HK; ++k) {
+                        if (!(odd[k >> 5] >> (k & 31) & 1u)) continue;
                         const unsigned* vp = reinterpret_cast<const unsigned*>(reinterpret_cast<const __half*>(P.v) + static_cast<size_t>(s) * P.v_seq +
                                                                                static_cast<size_t>(kvh) * P.v_head + static_cast<size_t>(t0 + k) * P.v_row);
-                        const unsigned ph = tc_ld1(ts + lanes + (k >> 1)) >> (16 * (k & 1)), pl = tc_ld1(ts + lanes + KT / 2 + (k >> 1)) >> (16 * (k & 1));
+                        const unsigned ph = tc_ld1(tp + (k >> 1)) >> (16 * (k & 1)), pl = tc_ld1(tp + HK / 2 + (k >> 1)) >> (16 * (k & 1));
                         const float p = half_bits_to_float(ph & 0xFFFFu) + half_bits_to_float(pl & 0xFFFFu);
                         if (p != 0.0f)
 #pragma unroll
-                            for (int ch = 0; ch < D / 2; ++ch) add_not_finite(o[2 * ch], o[2 * ch + 1], p, vp[ch]);
+                            for (int ch = 0; ch < D / 2; ++ch) add_not_finite(o[ch].x, o[ch].y, p, vp[ch]);
                         __syncwarp();
                     }
                 }
             }
             tc_before_sync();
-            named_sync(1 + wg, 128);
-            const int after = next(next(tile));
-            if (elected) {
-                tc_after_sync();
-                if (!*fail) issue_values(i);
-                if (after < nt) tc_wait(&full[(i + 2) % C::kStages], ((i + 2) / C::kStages) & 1, fail);
-            }
-            tc_wait(&ofull[wg], round & 1, fail);
-            tc_after_sync();
-            if (elected && after < nt && !*fail) issue_scores(i + 2);
+            bar_arrive(&pfull[wg]);
+        }
+        if (i > i0) {
+            tc_wait(&ofull[wg], (i - 1) & 1, fail);
             __syncwarp();
+            tc_after_sync();
+            drain();
+        }
+        if (FMT != 16) break;
+        float2 bad = make_float2(l * 0.0f, 0.0f);  // NaN if anything is not finite
 #pragma unroll
-            for (int h = 0; h < D / 32; ++h) {
-                float v[32];
-                tc_ld32(to + lanes + h * 32, v);
-                tc_ld_wait(v);
-#pragma unroll
-                for (int k = 0; k < 32; ++k) o[h * 32 + k] = fmaf(o[h * 32 + k], al, v[k]);
-            }
-            tc_before_sync();  // the next value products overwrite what was read: ordered by the warpgroup's barrier above
-            tile = after;
+        for (int k = 0; k < D / 2; ++k) bad = fma2(o[k], both(0.0f), bad);
+        if (!__syncthreads_or(!(bad.x + bad.y == 0.0f)) || careful) break;
         }
         // ---- the two warpgroups' sums joined: each finishes half of the channels ----------------------------------------------
         named_sync(4, 256);
-        float* ex = reinterpret_cast<float*>(sm);                          // [D / 2][128] of either half
-        float2* exml = reinterpret_cast<float2*>(sm + 128 * D * 4);        // [2][128]
+        float* ex = reinterpret_cast<float*>(sm + C::kOffK);                       // [D / 2][128] of either half
+        float2* exml = reinterpret_cast<float2*>(sm + C::kOffK + 128 * D * 4);     // [2][128]
         exml[wg * 128 + r] = make_float2(m, l);
 #pragma unroll
-        for (int i = 0; i < D / 2; ++i) ex[((wg ? 0 : D / 2) + i) * 128 + r] = wg ? o[i] : o[D / 2 + i];
+        for (int k = 0; k < D / 4; ++k) {
+            const float2 v = wg ? o[k] : o[D / 4 + k];
+            ex[((wg ? 0 : D / 2) + 2 * k) * 128 + r] = v.x;
+            ex[((wg ? 0 : D / 2) + 2 * k + 1) * 128 + r] = v.y;
+        }
         named_sync(4, 256);
         const float2 other = exml[(1 - wg) * 128 + r];
         const float M = fmaxf(m, other.x);
@@ -547,15 +639,11 @@ __global__ void __launch_bounds__(384, 1) attn_tc_kernel(const __grid_constant__
             }
             const float a = f0 * f, b = f1 * f;
 #pragma unroll
-            for (int i = 0; i < D / 2; i += 4) {
-                float4 v;
-                float* vp = &v.x;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float mine = wg ? o[D / 2 + i + k] : o[i + k];
-                    vp[k] = fmaf(mine, a, ex[(wg * (D / 2) + i + k) * 128 + r] * b);
-                }
-                *reinterpret_cast<float4*>(dst + wg * (D / 2) + i) = v;
+            for (int k = 0; k < D / 4; k += 2) {
+                const float2 x = wg ? o[D / 4 + k] : o[k], y = wg ? o[D / 4 + k + 1] : o[k + 1];
+                const float* e = ex + (wg * (D / 2) + 2 * k) * 128 + r;
+                *reinterpret_cast<float4*>(dst + wg * (D / 2) + 2 * k) =
+                    make_float4(fmaf(x.x, a, e[0] * b), fmaf(x.y, a, e[128] * b), fmaf(y.x, a, e[256] * b), fmaf(y.y, a, e[384] * b));
             }
             if (wg == 0) {
                 if (P.nsplit > 1) P.part_ml[part] = make_float2(M, L);
@@ -571,21 +659,43 @@ __global__ void __launch_bounds__(384, 1) attn_tc_kernel(const __grid_constant__
     tc_before_sync();
     __syncthreads();
     tc_after_sync();
-    if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    if (warp == C::kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 
+// Tensor map of an fp16 cache's keys or values: {channel, head, slot, sequence}, boxes of 64 channels x KT slots, 128-byte swizzle.
+inline bool cache_map(CUtensorMap* map, const uint8_t* base, const AttnP& P, int head_dim, long long row, long long head, long long seq, int slots) {
+    using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) p = nullptr;
+        return reinterpret_cast<Encode>(p);
+    }();
+    if (!encode) return false;
+    // a dimension of one element is never stepped over: its stride may be anything that is allowed
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(P.kv_heads), static_cast<cuuint64_t>(P.cap), static_cast<cuuint64_t>(P.n_seqs)};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(P.kv_heads > 1 ? head * 2 : 16), static_cast<cuuint64_t>(P.cap > 1 ? row * 2 : 16),
+                                   static_cast<cuuint64_t>(P.n_seqs > 1 ? seq * 2 : 16)};
+    const cuuint32_t box[4] = {64, 1, static_cast<cuuint32_t>(slots), 1}, one[4] = {1, 1, 1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<uint8_t*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 template <int D, int FMT>
 int attn_launch_tc(const AttnP& P, bool general, cudaStream_t st) {
     if constexpr (D == 64 || D == 128) {
-        constexpr int smem = TcCfg<D, FMT>::kSmem;
+        using C = TcCfg<D, FMT>;
+        CUtensorMap mk{}, mv{};
+        if (FMT == 16 && !(cache_map(&mk, P.k, P, D, P.k_row, P.k_head, P.k_seq, C::KT) && cache_map(&mv, P.v, P, D, P.v_row, P.v_head, P.v_seq, C::KT)))
+            return KCB_UNSUPPORTED_OPERATION;
         static PerDeviceFlag raised[2];
         const dim3 grid(P.row_tiles * P.nsplit, P.kv_heads, P.n_seqs);
         if (general) {
-            if (!raise_dynamic_smem(attn_tc_kernel<D, FMT, true>, smem, raised[0])) return KCB_LAUNCH_FAILURE;
-            attn_tc_kernel<D, FMT, true><<<grid, 384, smem, st>>>(P);
+            if (!raise_dynamic_smem(attn_tc_kernel<D, FMT, true>, C::kSmem, raised[0])) return KCB_LAUNCH_FAILURE;
+            attn_tc_kernel<D, FMT, true><<<grid, C::kThreads, C::kSmem, st>>>(P, mk, mv);
         } else {
-            if (!raise_dynamic_smem(attn_tc_kernel<D, FMT, false>, smem, raised[1])) return KCB_LAUNCH_FAILURE;
-            attn_tc_kernel<D, FMT, false><<<grid, 384, smem, st>>>(P);
+            if (!raise_dynamic_smem(attn_tc_kernel<D, FMT, false>, C::kSmem, raised[1])) return KCB_LAUNCH_FAILURE;
+            attn_tc_kernel<D, FMT, false><<<grid, C::kThreads, C::kSmem, st>>>(P, mk, mv);
         }
         return launch_status();
     }

@@ -558,7 +558,7 @@ int kcb_cache_attention(const kcb_kv_cache* c, const kcb_cache_attn* a, const fl
     ws += cut.ml_bytes + cut.o_bytes;
     P.final_ml = cut.final_bytes ? reinterpret_cast<float2*>(ws) : nullptr;
     P.scores = cut.score_bytes ? reinterpret_cast<float*>(ws) : nullptr;
-    const bool general = a->softcap > 0.0f || a->max_bias > 0.0f || c->positions || a->q_pos || a->q_doc || a->mask || a->prefix;
+    const bool general = a->softcap > 0.0f || a->max_bias > 0.0f || c->positions || a->q_doc || a->mask || ((a->q_pos || a->prefix) && cut.which != AttnKernel::tc);
     const auto st = static_cast<cudaStream_t>(stream);
     return attn_launch_bits(P, c->bits, c->head_dim, general, cut.which, st);
 }

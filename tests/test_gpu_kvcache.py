@@ -269,6 +269,17 @@ def test_strided_queries_outputs_and_caches(bits):
             assert torch.equal(kvcache.Attention(c2, n_tokens=N, heads=H)(q), want)
 
 
+@pytest.mark.parametrize("N", [1, 20, 100])
+def test_sequences_that_share_one_cache(N):
+    """A sequence stride of zero: one cache (a common system prompt) for all sequences."""
+    S, H, Hkv, D, cap = 3, 4, 2, 64, 200
+    c, k, v, gen = filled(16, 1, cap, Hkv, D, [200], seed=3)
+    n = torch.tensor([200, 150, 37], dtype=torch.int32, device="cuda")
+    shared = kvcache.KVCache(c.k.expand(S, -1, -1, -1), c.v.expand(S, -1, -1, -1), kv_heads=Hkv, head_dim=D, capacity=cap, n_keys=n, next_pos=n)
+    q = torch.randn(S, N, H, D, generator=gen, device="cuda")
+    check(shared, k.expand(S, -1, -1, -1), v.expand(S, -1, -1, -1), q, N, H)
+
+
 def test_offsets_past_32_bits():
     """Slots whose byte offsets pass 2^32 (4 bits) and whose element offsets pass 2^31 (fp16)."""
     Hkv, D = 1, 256
