@@ -29,14 +29,15 @@ namespace kcb {
 
 static __device__ unsigned g_attn_timeouts = 0;
 
-template <int D, int FMT>
+template <int D, int FMT, bool GEN>
 struct TcCfg {
-    static constexpr int HK = FMT == 16 ? 64 : 32;             // keys of a tile per softmax warpgroup
+    // keys of a tile per softmax warpgroup: 64 where a thread's scores and D outputs fit into its registers
+    static constexpr int HK = FMT == 16 && !(GEN && D == 128) ? 64 : 32;
     static constexpr int KT = 2 * HK, kRows = 128;
     static constexpr int kThreads = FMT == 16 ? 384 : 512, kMmaWarp = kThreads / 32 - 1, kProducers = kThreads - 256 - 32;
     static constexpr int kPlane = KT * D * 2;                  // one fp16 tile: D / 64 atoms of KT keys x 128 bytes
     static constexpr int kSlot = (FMT == 16 ? 1 : 2) * kPlane; // keys or values of a tile (4 bits: hi, lo)
-    static constexpr int kStages = D == 64 ? 4 : 2;            // of keys, and of values
+    static constexpr int kStages = kSlot > 16384 ? 2 : 4;      // of keys, and of values
     static constexpr int kQHalf = kRows * D * 2;               // hi, then lo queries
     static constexpr int kOffK = 2 * kQHalf, kOffV = kOffK + kStages * kSlot;
     static constexpr int kMeta = kOffV + kStages * kSlot;      // per stage: KT positions, KT documents, 16 bytes free, bits of odd slots
@@ -56,22 +57,27 @@ __device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t lbo) {  // 1
            (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
 }
 // D (TMEM, fp32) (+)= A B, fp16: A in shared memory or in TMEM, B in shared memory
+// The whole warp comes here, so that addresses and descriptors live in uniform registers; one elected lane issues (a branch to a
+// single lane instead made each product take 155 cycles to issue, against 64 to compute).
 __device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 __device__ __forceinline__ void tc_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    asm volatile(
+        "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
+        : "memory");
 }
 __device__ __forceinline__ void tc_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -119,6 +125,8 @@ __device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile
     return false;
 }
 
+// One answer for the whole warp.
+__device__ __forceinline__ bool warp_failed(volatile int* fail) { return __any_sync(0xffffffffu, *fail != 0); }
 // Packed fp32 pairs (one instruction for two values, each rounded as the scalar operation).
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     unsigned long long r;
@@ -135,39 +143,47 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
     return reinterpret_cast<float2&>(r);
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
 // Capped scores: y = tanh(u) cap, u = y on entry.  The power series below 0.55 (see tanh_series), elsewhere 1 - 2 / (e^2|u| + 1): there
 // the difference costs one bit.  A warp whose scores are all small against the cap, as most are, takes the series alone.
-template <int N>
-__device__ __forceinline__ void cap_scores(float (&y)[N], float cap) {
+template <int H>
+__device__ __forceinline__ void cap_scores(float (&y)[H][32], float cap) {
     float big = 0.0f;
 #pragma unroll
-    for (int k = 0; k < N; ++k) big = fmaxf(big, fabsf(y[k]));
+    for (int h = 0; h < H; ++h)
+#pragma unroll
+        for (int k = 0; k < 32; ++k) big = fmaxf(big, fabsf(y[h][k]));
     const bool small = __all_sync(0xffffffffu, big < 0.55f);
 #pragma unroll
-    for (int k = 0; k < N; k += 2) {
-        const float2 u = make_float2(y[k], y[k + 1]), w = mul2(u, u);
-        float2 r = fma2(both(-1.4558344e-3f), w, both(3.5921280e-3f));
-        r = fma2(r, w, both(-8.8632355e-3f));
-        r = fma2(r, w, both(2.1869488e-2f));
-        r = fma2(r, w, both(-5.3968254e-2f));
-        r = fma2(r, w, both(1.3333333e-1f));
-        r = fma2(r, w, both(-3.3333333e-1f));
-        r = fma2(mul2(u, w), r, u);
-        if (!small) {
-            if (fabsf(u.x) >= 0.55f) r.x = copysignf(1.0f - __fdividef(2.0f, ex2(2.0f * kLog2e * fabsf(u.x)) + 1.0f), u.x);
-            if (fabsf(u.y) >= 0.55f) r.y = copysignf(1.0f - __fdividef(2.0f, ex2(2.0f * kLog2e * fabsf(u.y)) + 1.0f), u.y);
+    for (int h = 0; h < H; ++h)
+#pragma unroll
+        for (int k = 0; k < 32; k += 2) {
+            const float2 u = make_float2(y[h][k], y[h][k + 1]), w = mul2(u, u);
+            float2 r = fma2(both(-1.4558344e-3f), w, both(3.5921280e-3f));
+            r = fma2(r, w, both(-8.8632355e-3f));
+            r = fma2(r, w, both(2.1869488e-2f));
+            r = fma2(r, w, both(-5.3968254e-2f));
+            r = fma2(r, w, both(1.3333333e-1f));
+            r = fma2(r, w, both(-3.3333333e-1f));
+            r = mul2(fma2(mul2(u, w), r, u), both(cap));
+            if (!small) {
+                if (fabsf(u.x) >= 0.55f) r.x = copysignf(cap - __fdividef(2.0f * cap, ex2(2.0f * kLog2e * fabsf(u.x)) + 1.0f), u.x);
+                if (fabsf(u.y) >= 0.55f) r.y = copysignf(cap - __fdividef(2.0f * cap, ex2(2.0f * kLog2e * fabsf(u.y)) + 1.0f), u.y);
+            }
+            y[h][k] = r.x, y[h][k + 1] = r.y;
         }
-        r = mul2(r, both(cap));
-        y[k] = r.x, y[k + 1] = r.y;
-    }
 }
 
 template <int D, int FMT, bool GEN>
-__global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
+__global__ void __launch_bounds__(TcCfg<D, FMT, GEN>::kThreads, 1)
     attn_tc_kernel(const __grid_constant__ AttnP P, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
-    using C = TcCfg<D, FMT>;
+    using C = TcCfg<D, FMT, GEN>;
     constexpr int HK = C::HK, KT = C::KT, NB = D / 32, CH = D / 8;
     extern __shared__ uint8_t sm_raw[];
     uint8_t* sm = sm_raw + ((1024u - (smem_u32(sm_raw) & 1023u)) & 1023u);
@@ -235,7 +251,8 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
         }
         float up, down;
         row_scale(amax, up, down);
-        ysc = P.sc * down;
+        ysc = fmaxf(fabsf(P.sc) * down, 1e-37f);  // positive, so that the largest product is the largest score; a negative scale goes to the query
+        if (P.sc < 0.0f) up = -up;
 #pragma unroll 4
         for (int ch = 0; ch < CH; ++ch) {
             const float4 a = valid ? qp[2 * ch] : zero, b = valid ? qp[2 * ch + 1] : zero;
@@ -251,7 +268,7 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
     tc_before_sync();
     __syncthreads();
     tc_after_sync();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     // (after an expired wait every loop below runs on, without products, so that every barrier finds its arrivals)
 
     if (wg >= 2) {
@@ -261,7 +278,7 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
             int i = 0;  // tiles so far, over both passes: stages and parities go by it
             for (bool careful = false;; careful = true) {
                 const int i0 = i;
-                if (lane == 0) {
+                {
                     const uint32_t base = smem_u32(sm);
                     constexpr uint32_t kIdescS = (1u << 4) | (static_cast<uint32_t>(KT >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
                     constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
@@ -269,8 +286,9 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
                     auto scores = [&](int j) {  // (hi + lo) keys^T, both halves of the tile
                         const int st = j % C::kStages;
                         tc_wait(&kfull[st], (j / C::kStages) & 1, fail);
+                        __syncwarp();
                         tc_after_sync();
-                        if (*fail) return;
+                        if (warp_failed(fail)) return;
                         const uint32_t kb = base + C::kOffK + st * C::kSlot;
 #pragma unroll
                         for (int k = 0; k < D / 16; ++k) {
@@ -295,8 +313,9 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
 #pragma unroll
                         for (int w = 0; w < 2; ++w) {
                             tc_wait(&pfull[w], i & 1, fail);
+                            __syncwarp();
                             tc_after_sync();
-                            if (*fail) continue;
+                            if (warp_failed(fail)) continue;
 #pragma unroll
                             for (int k = 0; k < HK / 16; ++k) {
                                 const uint32_t ph = tmem + C::kP + w * HK + k * 8, pl = ph + HK / 2, od = tmem + C::kO + w * D;
@@ -307,7 +326,7 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
                             }
                             tc_commit(&ofull[w]);
                         }
-                        if (!*fail) tc_commit(&vempty[st]);
+                        if (!warp_failed(fail)) tc_commit(&vempty[st]);
                         ++i;
                     }
                 }
@@ -441,13 +460,14 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
         float2 o[D / 2];
         float m, l, al;
         auto drain = [&]() {  // o = o al + the last tile's output
+            float v[2][32];  // the next 32 channels are on their way while these are added
+            tc_ld32(to, v[0]);
 #pragma unroll
             for (int h = 0; h < D / 32; ++h) {
-                float v[32];
-                tc_ld32(to + h * 32, v);
-                tc_ld_wait(v);
+                tc_ld_wait(v[h & 1]);
+                if (h + 1 < D / 32) tc_ld32(to + (h + 1) * 32, v[(h + 1) & 1]);
 #pragma unroll
-                for (int k = 0; k < 16; ++k) o[h * 16 + k] = fma2(o[h * 16 + k], both(al), make_float2(v[2 * k], v[2 * k + 1]));
+                for (int k = 0; k < 16; ++k) o[h * 16 + k] = fma2(o[h * 16 + k], both(al), make_float2(v[h & 1][2 * k], v[h & 1][2 * k + 1]));
             }
         };
         int i = 0;  // tiles so far, over both passes
@@ -463,20 +483,21 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
             tc_wait(sfull, i & 1, fail);
             __syncwarp();
             tc_after_sync();
-            float y[HK];
-            tc_ld32(ts, reinterpret_cast<float(&)[32]>(y[0]));
-            if (HK == 64) tc_ld32(ts + 32, reinterpret_cast<float(&)[32]>(y[HK - 32]));
-            tc_ld_wait(reinterpret_cast<float(&)[32]>(y[0]));
-            if (HK == 64) tc_ld_wait(reinterpret_cast<float(&)[32]>(y[HK - 32]));
+            float yy[HK / 32][32];
+#pragma unroll
+            for (int h = 0; h < HK / 32; ++h) tc_ld32(ts + h * 32, yy[h]);
+#pragma unroll
+            for (int h = 0; h < HK / 32; ++h) tc_ld_wait(yy[h]);
+#define Y(k) yy[(k) >> 5][(k) & 31]
             tc_before_sync();
             bar_arrive(sread);
-#pragma unroll
-            for (int k = 0; k < HK; k += 2) {
-                const float2 t = mul2(make_float2(y[k], y[k + 1]), both(ysc));
-                y[k] = t.x, y[k + 1] = t.y;
-            }
             if (GEN) {
-                if (P.cap_out != 0.0f) cap_scores(y, P.cap_out);
+#pragma unroll
+                for (int k = 0; k < HK; k += 2) {
+                    const float2 t = mul2(make_float2(Y(k), Y(k + 1)), both(ysc));
+                    Y(k) = t.x, Y(k + 1) = t.y;
+                }
+                if (P.cap_out != 0.0f) cap_scores(yy, P.cap_out);
                 if (P.positions || P.k_doc) tc_wait(FMT == 16 ? &mfull[st] : &vfull[st], (i / C::kStages) & 1, fail);
                 if (P.mask) {
                     const unsigned short* mp = ri.mask + t0;
@@ -496,7 +517,7 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
                         }
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
-                            float& v = y[k8 * 8 + k];
+                            float& v = Y(k8 * 8 + k);
                             const unsigned h = w[k >> 1] >> (16 * (k & 1)) & 0xFFFFu;
                             v = h == 0xFC00u ? -INFINITY : fmaf(ri.slope, half_bits_to_float(h), v);
                         }
@@ -505,42 +526,46 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
                     const float qp = static_cast<float>(ri.pos);
                     if (P.positions) {
 #pragma unroll
-                        for (int k = 0; k < HK; ++k) y[k] -= ri.slope * fabsf(qp - static_cast<float>(meta[k]));
+                        for (int k = 0; k < HK; ++k) Y(k) -= ri.slope * fabsf(qp - static_cast<float>(meta[k]));
                     } else {
                         const float far = static_cast<float>(ri.pos) - static_cast<float>(t0);
 #pragma unroll
-                        for (int k = 0; k < HK; ++k) y[k] -= ri.slope * fabsf(far - static_cast<float>(k));
+                        for (int k = 0; k < HK; ++k) Y(k) -= ri.slope * fabsf(far - static_cast<float>(k));
                     }
                 }
                 if (P.causal && P.positions) {
 #pragma unroll
                     for (int k = 0; k < HK; k += 4) {
                         const int4 kp = *reinterpret_cast<const int4*>(meta + k);
-                        if (kp.x > ri.pos && kp.x >= prefix) y[k] = -INFINITY;
-                        if (kp.y > ri.pos && kp.y >= prefix) y[k + 1] = -INFINITY;
-                        if (kp.z > ri.pos && kp.z >= prefix) y[k + 2] = -INFINITY;
-                        if (kp.w > ri.pos && kp.w >= prefix) y[k + 3] = -INFINITY;
+                        if (kp.x > ri.pos && kp.x >= prefix) Y(k) = -INFINITY;
+                        if (kp.y > ri.pos && kp.y >= prefix) Y(k + 1) = -INFINITY;
+                        if (kp.z > ri.pos && kp.z >= prefix) Y(k + 2) = -INFINITY;
+                        if (kp.w > ri.pos && kp.w >= prefix) Y(k + 3) = -INFINITY;
                     }
                 }
                 if (docs) {
 #pragma unroll
                     for (int k = 0; k < HK; k += 4) {
                         const int4 kd = *reinterpret_cast<const int4*>(meta + KT + k);
-                        if (kd.x != ri.doc) y[k] = -INFINITY;
-                        if (kd.y != ri.doc) y[k + 1] = -INFINITY;
-                        if (kd.z != ri.doc) y[k + 2] = -INFINITY;
-                        if (kd.w != ri.doc) y[k + 3] = -INFINITY;
+                        if (kd.x != ri.doc) Y(k) = -INFINITY;
+                        if (kd.y != ri.doc) Y(k + 1) = -INFINITY;
+                        if (kd.z != ri.doc) Y(k + 2) = -INFINITY;
+                        if (kd.w != ri.doc) Y(k + 3) = -INFINITY;
                     }
                 }
             }
             if (!__all_sync(0xffffffffu, t0 + HK <= limit)) {
 #pragma unroll
                 for (int k = 0; k < HK; ++k)
-                    if (t0 + k >= limit) y[k] = -INFINITY;
+                    if (t0 + k >= limit) Y(k) = -INFINITY;
             }
-            float mx = m;
+            float mx = Y(0), mx1 = Y(1);
 #pragma unroll
-            for (int k = 0; k < HK; k += 2) mx = fmaxf(mx, fmaxf(y[k], y[k + 1]));
+            for (int k = 2; k < HK; k += 4) {
+                mx = max3(mx, Y(k), Y(k + 1));
+                if (k + 2 < HK) mx1 = max3(mx1, Y(k + 2), Y(k + 3));
+            }
+            mx = max3(m, fmaxf(mx, mx1) * (GEN ? 1.0f : ysc), -INFINITY);
             const float al1 = mx > m ? ex2(m - mx) : 1.0f;
             m = mx;
             const float2 ref = both(m == -INFINITY ? 0.0f : kPShift - m);
@@ -556,17 +581,18 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
                 unsigned hi[16], lo[16];
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
-                    const float2 e = add2(make_float2(y[h * 32 + 2 * k], y[h * 32 + 2 * k + 1]), ref);
+                    const float2 v = make_float2(yy[h][2 * k], yy[h][2 * k + 1]), e = GEN ? add2(v, ref) : fma2(v, both(ysc), ref);
                     const float2 p = make_float2(ex2(e.x), ex2(e.y));
                     if (k & 1) sum1 = add2(sum1, p);
                     else sum = add2(sum, p);
                     const __half2 hh = __floats2half2_rn(p.x, p.y);
-                    const float2 f = __half22float2(hh), d = add2(p, make_float2(-f.x, -f.y));
+                    const float2 d = fma2(__half22float2(hh), both(-1.0f), p);
                     hi[k] = h2_bits(hh), lo[k] = h2_bits(__floats2half2_rn(d.x, d.y));
                 }
                 tc_st16(tp + h * 16, hi);
                 tc_st16(tp + HK / 2 + h * 16, lo);
             }
+#undef Y
             sum = add2(sum, sum1);
             l = fmaf(l, al1, sum.x + sum.y);
             if (i > i0) drain();
@@ -684,9 +710,11 @@ inline bool cache_map(CUtensorMap* map, const uint8_t* base, const AttnP& P, int
 template <int D, int FMT>
 int attn_launch_tc(const AttnP& P, bool general, cudaStream_t st) {
     if constexpr (D == 64 || D == 128) {
-        using C = TcCfg<D, FMT>;
+        using C = TcCfg<D, FMT, true>;
+        using N = TcCfg<D, FMT, false>;
+        const int slots = general ? C::KT : N::KT;
         CUtensorMap mk{}, mv{};
-        if (FMT == 16 && !(cache_map(&mk, P.k, P, D, P.k_row, P.k_head, P.k_seq, C::KT) && cache_map(&mv, P.v, P, D, P.v_row, P.v_head, P.v_seq, C::KT)))
+        if (FMT == 16 && !(cache_map(&mk, P.k, P, D, P.k_row, P.k_head, P.k_seq, slots) && cache_map(&mv, P.v, P, D, P.v_row, P.v_head, P.v_seq, slots)))
             return KCB_UNSUPPORTED_OPERATION;
         static PerDeviceFlag raised[2];
         const dim3 grid(P.row_tiles * P.nsplit, P.kv_heads, P.n_seqs);
@@ -694,8 +722,8 @@ int attn_launch_tc(const AttnP& P, bool general, cudaStream_t st) {
             if (!raise_dynamic_smem(attn_tc_kernel<D, FMT, true>, C::kSmem, raised[0])) return KCB_LAUNCH_FAILURE;
             attn_tc_kernel<D, FMT, true><<<grid, C::kThreads, C::kSmem, st>>>(P, mk, mv);
         } else {
-            if (!raise_dynamic_smem(attn_tc_kernel<D, FMT, false>, C::kSmem, raised[1])) return KCB_LAUNCH_FAILURE;
-            attn_tc_kernel<D, FMT, false><<<grid, C::kThreads, C::kSmem, st>>>(P, mk, mv);
+            if (!raise_dynamic_smem(attn_tc_kernel<D, FMT, false>, N::kSmem, raised[1])) return KCB_LAUNCH_FAILURE;
+            attn_tc_kernel<D, FMT, false><<<grid, N::kThreads, N::kSmem, st>>>(P, mk, mv);
         }
         return launch_status();
     }
