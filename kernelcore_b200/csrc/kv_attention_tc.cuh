@@ -3,16 +3,17 @@
 // cache exact as it is; 4-bit values d code + m (a multiple of 2^-24, as every fp16 number is) as hi + lo pairs too, of whose four
 // products with a query or probability the smallest, lo * lo (2^-22), is left out.
 //
-// Three warpgroups.
+// Roles.
 //   * Two softmax warpgroups, one query row per thread in each: a tile of keys is cut into halves, and each warpgroup has its half of
-//     every tile, with its own running maximum, sum and output, joined at the end.  Per tile a thread reads its row's scores from
-//     TMEM, turns them into probabilities and stores those, as hi and lo halves, to TMEM, the A operand of the value products.
+//     every tile's scores.  A thread reads its row's scores from TMEM, exchanges their maximum with the thread that has the other half
+//     of the row, turns them into probabilities and stores those, as hi and lo halves, to TMEM, the A operand of the value products.
 //   * The rest: one warp issues all products -- scores of the next tile as soon as both warpgroups have read this one's, so that they
 //     run under the softmax -- and the others bring keys and values into rings of stages in the 128-byte-swizzled layout of the
 //     operands: fp16 rows by tensor copies that one thread issues, 4-bit rows unpacked through registers.
-//   * A tile's output starts from zero in TMEM and is added to the thread's running output in registers, in fp32: no rescaling in
-//     TMEM, and the length of the context never meets the truncation of the tensor cores' sums.
-// TMEM (512 columns at D = 128, fp16): scores of both halves 2 * 64, probabilities 2 * 64, outputs 2 * 128.
+//   * A tile's output starts from zero in TMEM and is added to running outputs in registers, in fp32, half of the channels by either
+//     warpgroup: no rescaling in TMEM, and the length of the context never meets the tensor cores' sums, which truncate (each product
+//     of K = 16 can cost its sum an ulp towards zero).
+// TMEM (512 columns at D = 128, fp16): 128 scores, two buffers of 128 probabilities (hi and lo, two to a column), 128 outputs.
 // Values that are not finite would reach rows that do not see them as 0 * inf, and so would what lies behind the rows in use, which
 // a tensor copy brings along.  Looking for such values costs a third of the kernel's time, so the first pass does not: where an output
 // is not finite at its end, the CTA takes a second pass that does, clears them from the tiles, and gives them to the rows that see
@@ -29,10 +30,9 @@ namespace kcb {
 
 static __device__ unsigned g_attn_timeouts = 0;
 
-template <int D, int FMT, bool GEN>
+template <int D, int FMT>
 struct TcCfg {
-    // keys of a tile per softmax warpgroup: 64 where a thread's scores and D outputs fit into its registers
-    static constexpr int HK = FMT == 16 && !(GEN && D == 128) ? 64 : 32;
+    static constexpr int HK = FMT == 16 ? 64 : 32;             // keys of a tile per softmax warpgroup
     static constexpr int KT = 2 * HK, kRows = 128;
     static constexpr int kThreads = FMT == 16 ? 384 : 512, kMmaWarp = kThreads / 32 - 1, kProducers = kThreads - 256 - 32;
     static constexpr int kPlane = KT * D * 2;                  // one fp16 tile: D / 64 atoms of KT keys x 128 bytes
@@ -42,14 +42,14 @@ struct TcCfg {
     static constexpr int kOffK = 2 * kQHalf, kOffV = kOffK + kStages * kSlot;
     static constexpr int kMeta = kOffV + kStages * kSlot;      // per stage: KT positions, KT documents, 16 bytes free, bits of odd slots
     static constexpr int kMetaBytes = 2 * KT * 4 + 32;
-    static constexpr int kBars = kMeta + kStages * kMetaBytes;
+    static constexpr int kMax = kMeta + kStages * kMetaBytes;  // maxima exchanged: [2][warpgroup][row]
+    static constexpr int kBars = kMax + 2 * 2 * kRows * 4;
     static constexpr int kTile0 = kBars + 256;                 // bitmap of tiles
     static constexpr int kSmem = kTile0 + kDocBits / 8 + 1024; // + room to align the base to 1024 bytes
-    static constexpr uint32_t kS = 0, kP = KT, kO = 2 * KT;    // TMEM columns
+    static constexpr uint32_t kS = 0, kP = KT, kO = 3 * KT;    // TMEM columns: scores, two buffers of probabilities, outputs
     static constexpr int kRegsSoftmax = FMT == 16 ? 224 : 184, kRegsProducer = FMT == 16 ? 56 : 72, kRegsLaunch = FMT == 16 ? 168 : 128;
     static_assert(2 * 128 * kRegsSoftmax + (kThreads - 256) * kRegsProducer <= kThreads * kRegsLaunch, "the softmax warpgroups take what the producers give up");
-    static_assert(kO + 2 * D <= 512 && kMetaBytes % 16 == 0 && kSmem <= kMaxSmem && kSmem > kMaxSmem / 2, "TMEM columns; one CTA per SM");
-    static_assert(128 * D * 4 + 2048 <= 2 * kStages * kSlot, "the exchange at the end reuses the rings");
+    static_assert(kO + D <= 512 && kMetaBytes % 16 == 0 && kSmem <= kMaxSmem && kSmem > kMaxSmem / 2, "TMEM columns; one CTA per SM");
 };
 
 __device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t lbo) {  // 128-byte swizzle, 8-row groups 1024 bytes apart
@@ -181,9 +181,9 @@ __device__ __forceinline__ void cap_scores(float (&y)[H][32], float cap) {
 }
 
 template <int D, int FMT, bool GEN>
-__global__ void __launch_bounds__(TcCfg<D, FMT, GEN>::kThreads, 1)
+__global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
     attn_tc_kernel(const __grid_constant__ AttnP P, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
-    using C = TcCfg<D, FMT, GEN>;
+    using C = TcCfg<D, FMT>;
     constexpr int HK = C::HK, KT = C::KT, NB = D / 32, CH = D / 8;
     extern __shared__ uint8_t sm_raw[];
     uint8_t* sm = sm_raw + ((1024u - (smem_u32(sm_raw) & 1023u)) & 1023u);
@@ -195,10 +195,11 @@ __global__ void __launch_bounds__(TcCfg<D, FMT, GEN>::kThreads, 1)
     uint64_t* mfull = varrived + C::kStages;                       // [stage] fp16: positions and documents written
     uint64_t* sfull = mfull + C::kStages;                          // scores of a tile complete
     uint64_t* sread = sfull + 1;                                   // ... and read by both warpgroups
-    uint64_t* pfull = sread + 1;                                   // [warpgroup] probabilities stored, last output read
-    uint64_t* ofull = pfull + 2;                                   // [warpgroup] output of a tile complete
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ofull + 2);
-    volatile int* fail = reinterpret_cast<volatile int*>(ofull + 3);
+    uint64_t* mxfull = sread + 1;                                  // a tile's maxima written
+    uint64_t* pfull = mxfull + 1;                                  // probabilities stored, last output read
+    uint64_t* ofull = pfull + 1;                                   // output of a tile complete
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ofull + 1);
+    volatile int* fail = reinterpret_cast<volatile int*>(ofull + 2);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wg = warp >> 2;
     const int rt = P.row_tiles - 1 - static_cast<int>(blockIdx.x) / P.nsplit, split = blockIdx.x % P.nsplit, kvh = blockIdx.y, s = blockIdx.z;
     const int row0 = rt * C::kRows;
@@ -218,8 +219,7 @@ __global__ void __launch_bounds__(TcCfg<D, FMT, GEN>::kThreads, 1)
             mbar_init(&kfull[i], FMT == 16 ? 1 : C::kProducers), mbar_init(&kempty[i], 1), mbar_init(&vfull[i], C::kProducers), mbar_init(&vempty[i], 1);
             mbar_init(&varrived[i], 1), mbar_init(&mfull[i], 64);
         }
-        mbar_init(sfull, 1), mbar_init(sread, 256);
-        for (int i = 0; i < 2; ++i) mbar_init(&pfull[i], 128), mbar_init(&ofull[i], 1);
+        mbar_init(sfull, 1), mbar_init(sread, 256), mbar_init(mxfull, 256), mbar_init(pfull, 256), mbar_init(ofull, 1);
         *fail = 0;
         mbar_init_fence();
     }
@@ -310,23 +310,21 @@ __global__ void __launch_bounds__(TcCfg<D, FMT, GEN>::kThreads, 1)
                         const int st = i % C::kStages;
                         const uint32_t vb = base + C::kOffV + st * C::kSlot;
                         tc_wait(&vready[st], ((i - (careful ? i0 : 0)) / C::kStages) & 1, fail);  // (vfull completes in the second pass alone)
+                        tc_wait(pfull, i & 1, fail);
+                        __syncwarp();
+                        tc_after_sync();
+                        if (!warp_failed(fail)) {
 #pragma unroll
-                        for (int w = 0; w < 2; ++w) {
-                            tc_wait(&pfull[w], i & 1, fail);
-                            __syncwarp();
-                            tc_after_sync();
-                            if (warp_failed(fail)) continue;
-#pragma unroll
-                            for (int k = 0; k < HK / 16; ++k) {
-                                const uint32_t ph = tmem + C::kP + w * HK + k * 8, pl = ph + HK / 2, od = tmem + C::kO + w * D;
-                                const uint64_t vd = tc_desc(vb + (w * HK + k * 16) * 128, KT * 128);
-                                tc_mma(od, ph, vd, kIdescO, k > 0);
-                                tc_mma(od, pl, vd, kIdescO, 1);
-                                if (FMT != 16) tc_mma(od, ph, vd + (C::kPlane >> 4), kIdescO, 1);
+                            for (int k = 0; k < KT / 16; ++k) {
+                                const uint32_t ph = tmem + C::kP + (i & 1) * KT + k * 8, pl = ph + KT / 2;
+                                const uint64_t vd = tc_desc(vb + k * 2048, KT * 128);
+                                tc_mma(tmem + C::kO, ph, vd, kIdescO, k > 0);
+                                tc_mma(tmem + C::kO, pl, vd, kIdescO, 1);
+                                if (FMT != 16) tc_mma(tmem + C::kO, ph, vd + (C::kPlane >> 4), kIdescO, 1);
                             }
-                            tc_commit(&ofull[w]);
+                            tc_commit(ofull);
+                            tc_commit(&vempty[st]);
                         }
-                        if (!warp_failed(fail)) tc_commit(&vempty[st]);
                         ++i;
                     }
                 }
@@ -450,22 +448,23 @@ __global__ void __launch_bounds__(TcCfg<D, FMT, GEN>::kThreads, 1)
         const int r = tid & 127, row = row0 + r;
         const bool valid = row < P.rows;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem + C::kS + wg * HK + lanes, tp = tmem + C::kP + wg * HK + lanes, to = tmem + C::kO + wg * D + lanes;
+        const uint32_t ts = tmem + C::kS + wg * HK + lanes, to = tmem + C::kO + wg * (D / 2) + lanes;
+        float* maxima = reinterpret_cast<float*>(sm + C::kMax);
         RowInfo ri{};
         if (GEN) ri = row_info(P, s, kvh, n, row);
         // slots from `limit` on are hidden by the end of the range, or (slot = position) by causality
         int limit = valid ? end : 0;
         if (P.causal && valid && !(GEN && P.positions)) limit = min(end, max(prefix, row_pos(P, s, n, row / P.group) + 1));
 
-        float2 o[D / 2];
+        float2 o[D / 4];  // this warpgroup's half of the channels
         float m, l, al;
         auto drain = [&]() {  // o = o al + the last tile's output
             float v[2][32];  // the next 32 channels are on their way while these are added
             tc_ld32(to, v[0]);
 #pragma unroll
-            for (int h = 0; h < D / 32; ++h) {
+            for (int h = 0; h < D / 64; ++h) {
                 tc_ld_wait(v[h & 1]);
-                if (h + 1 < D / 32) tc_ld32(to + (h + 1) * 32, v[(h + 1) & 1]);
+                if (h + 1 < D / 64) tc_ld32(to + (h + 1) * 32, v[(h + 1) & 1]);
 #pragma unroll
                 for (int k = 0; k < 16; ++k) o[h * 16 + k] = fma2(o[h * 16 + k], both(al), make_float2(v[h & 1][2 * k], v[h & 1][2 * k + 1]));
             }
@@ -475,7 +474,7 @@ __global__ void __launch_bounds__(TcCfg<D, FMT, GEN>::kThreads, 1)
         const int i0 = i;
         m = -INFINITY, l = 0.0f, al = 1.0f;
 #pragma unroll
-        for (int k = 0; k < D / 2; ++k) o[k] = make_float2(0.0f, 0.0f);
+        for (int k = 0; k < D / 4; ++k) o[k] = make_float2(0.0f, 0.0f);
         for (int tile = next(-1); tile < nt; tile = next(tile), ++i) {
             const int t0 = begin + tile * KT + wg * HK;  // this warpgroup's first slot
             const int st = i % C::kStages;
@@ -565,17 +564,17 @@ __global__ void __launch_bounds__(TcCfg<D, FMT, GEN>::kThreads, 1)
                 mx = max3(mx, Y(k), Y(k + 1));
                 if (k + 2 < HK) mx1 = max3(mx1, Y(k + 2), Y(k + 3));
             }
-            mx = max3(m, fmaxf(mx, mx1) * (GEN ? 1.0f : ysc), -INFINITY);
+            mx = fmaxf(mx, mx1) * (GEN ? 1.0f : ysc);
+            maxima[((i & 1) * 2 + wg) * C::kRows + r] = mx;
+            bar_arrive(mxfull);
+            tc_wait(mxfull, i & 1, fail);
+            mx = max3(m, mx, maxima[((i & 1) * 2 + 1 - wg) * C::kRows + r]);
             const float al1 = mx > m ? ex2(m - mx) : 1.0f;
             m = mx;
             const float2 ref = both(m == -INFINITY ? 0.0f : kPShift - m);
             float2 sum = make_float2(0.0f, 0.0f), sum1 = sum;
-            // the last tile's value products have read their probabilities: this tile's may take the place
-            if (i > i0) {
-                tc_wait(&ofull[wg], (i - 1) & 1, fail);
-                __syncwarp();
-                tc_after_sync();
-            }
+            const uint32_t tp = tmem + C::kP + (i & 1) * KT + wg * (HK / 2) + lanes;
+            __syncwarp();
 #pragma unroll
             for (int h = 0; h < HK / 32; ++h) {
                 unsigned hi[16], lo[16];
@@ -590,42 +589,51 @@ __global__ void __launch_bounds__(TcCfg<D, FMT, GEN>::kThreads, 1)
                     hi[k] = h2_bits(hh), lo[k] = h2_bits(__floats2half2_rn(d.x, d.y));
                 }
                 tc_st16(tp + h * 16, hi);
-                tc_st16(tp + HK / 2 + h * 16, lo);
+                tc_st16(tp + KT / 2 + h * 16, lo);
             }
 #undef Y
             sum = add2(sum, sum1);
             l = fmaf(l, al1, sum.x + sum.y);
-            if (i > i0) drain();
+            if (i > i0) {
+                tc_wait(ofull, (i - 1) & 1, fail);
+                __syncwarp();
+                tc_after_sync();
+                drain();
+            }
             al = al1;
             tc_st_wait();
             if (FMT == 16 && careful) {  // values of this tile that are not finite go to the rows that see them one by one
                 tc_wait(&vfull[st], ((i - i0) / C::kStages) & 1, fail);
-                const unsigned* odd = reinterpret_cast<const unsigned*>(sm + C::kMeta + st * C::kMetaBytes + 2 * KT * 4 + 16) + wg * (HK / 32);
+                const unsigned* odd = reinterpret_cast<const unsigned*>(sm + C::kMeta + st * C::kMetaBytes + 2 * KT * 4 + 16);
                 unsigned any = 0;
 #pragma unroll
-                for (int h = 0; h < HK / 32; ++h) any |= odd[h];
-                __syncwarp();
+                for (int h = 0; h < KT / 32; ++h) any |= odd[h];
+                tc_before_sync();
+                named_sync(4, 256);  // both halves of the probabilities are stored
+                tc_after_sync();
                 if (any) {
                     al = fmaxf(al, 1e-30f);  // an infinity added now stays one when the output is rescaled
+                    const uint32_t pb = tmem + C::kP + (i & 1) * KT + lanes;
+                    const int first = begin + tile * KT;
 #pragma unroll 1
-                    for (int k = 0; k < HK; ++k) {
+                    for (int k = 0; k < KT; ++k) {
                         if (!(odd[k >> 5] >> (k & 31) & 1u)) continue;
                         const unsigned* vp = reinterpret_cast<const unsigned*>(reinterpret_cast<const __half*>(P.v) + static_cast<size_t>(s) * P.v_seq +
-                                                                               static_cast<size_t>(kvh) * P.v_head + static_cast<size_t>(t0 + k) * P.v_row);
-                        const unsigned ph = tc_ld1(tp + (k >> 1)) >> (16 * (k & 1)), pl = tc_ld1(tp + HK / 2 + (k >> 1)) >> (16 * (k & 1));
+                                                                               static_cast<size_t>(kvh) * P.v_head + static_cast<size_t>(first + k) * P.v_row + wg * (D / 2));
+                        const unsigned ph = tc_ld1(pb + (k >> 1)) >> (16 * (k & 1)), pl = tc_ld1(pb + KT / 2 + (k >> 1)) >> (16 * (k & 1));
                         const float p = half_bits_to_float(ph & 0xFFFFu) + half_bits_to_float(pl & 0xFFFFu);
                         if (p != 0.0f)
 #pragma unroll
-                            for (int ch = 0; ch < D / 2; ++ch) add_not_finite(o[ch].x, o[ch].y, p, vp[ch]);
+                            for (int ch = 0; ch < D / 4; ++ch) add_not_finite(o[ch].x, o[ch].y, p, vp[ch]);
                         __syncwarp();
                     }
                 }
             }
             tc_before_sync();
-            bar_arrive(&pfull[wg]);
+            bar_arrive(pfull);
         }
         if (i > i0) {
-            tc_wait(&ofull[wg], (i - 1) & 1, fail);
+            tc_wait(ofull, (i - 1) & 1, fail);
             __syncwarp();
             tc_after_sync();
             drain();
@@ -633,25 +641,14 @@ __global__ void __launch_bounds__(TcCfg<D, FMT, GEN>::kThreads, 1)
         if (FMT != 16) break;
         float2 bad = make_float2(l * 0.0f, 0.0f);  // NaN if anything is not finite
 #pragma unroll
-        for (int k = 0; k < D / 2; ++k) bad = fma2(o[k], both(0.0f), bad);
+        for (int k = 0; k < D / 4; ++k) bad = fma2(o[k], both(0.0f), bad);
         if (!__syncthreads_or(!(bad.x + bad.y == 0.0f)) || careful) break;
         }
-        // ---- the two warpgroups' sums joined: each finishes half of the channels ----------------------------------------------
+        // ---- the row's sum over both halves of its keys; each warpgroup stores its half of the channels ---------------------------
         named_sync(4, 256);
-        float* ex = reinterpret_cast<float*>(sm + C::kOffK);                       // [D / 2][128] of either half
-        float2* exml = reinterpret_cast<float2*>(sm + C::kOffK + 128 * D * 4);     // [2][128]
-        exml[wg * 128 + r] = make_float2(m, l);
-#pragma unroll
-        for (int k = 0; k < D / 4; ++k) {
-            const float2 v = wg ? o[k] : o[D / 4 + k];
-            ex[((wg ? 0 : D / 2) + 2 * k) * 128 + r] = v.x;
-            ex[((wg ? 0 : D / 2) + 2 * k + 1) * 128 + r] = v.y;
-        }
+        maxima[wg * C::kRows + r] = l;
         named_sync(4, 256);
-        const float2 other = exml[(1 - wg) * 128 + r];
-        const float M = fmaxf(m, other.x);
-        const float f0 = l != 0.0f ? ex2(m - M) : 0.0f, f1 = other.y != 0.0f ? ex2(other.x - M) : 0.0f;
-        const float L = (l != 0.0f ? l * f0 : 0.0f) + (other.y != 0.0f ? other.y * f1 : 0.0f);
+        const float L = l + maxima[(1 - wg) * C::kRows + r];
         const size_t part = ((static_cast<size_t>(s) * P.kv_heads + kvh) * P.nsplit + split) * P.rows + row;
         if (valid) {
             float* dst;
@@ -663,17 +660,11 @@ __global__ void __launch_bounds__(TcCfg<D, FMT, GEN>::kThreads, 1)
                 const int token = row / P.group, head = kvh * P.group + row % P.group;
                 dst = P.out + static_cast<size_t>(s) * P.o_seq + static_cast<size_t>(token) * P.o_token + static_cast<size_t>(head) * P.o_head;
             }
-            const float a = f0 * f, b = f1 * f;
 #pragma unroll
-            for (int k = 0; k < D / 4; k += 2) {
-                const float2 x = wg ? o[D / 4 + k] : o[k], y = wg ? o[D / 4 + k + 1] : o[k + 1];
-                const float* e = ex + (wg * (D / 2) + 2 * k) * 128 + r;
-                *reinterpret_cast<float4*>(dst + wg * (D / 2) + 2 * k) =
-                    make_float4(fmaf(x.x, a, e[0] * b), fmaf(x.y, a, e[128] * b), fmaf(y.x, a, e[256] * b), fmaf(y.y, a, e[384] * b));
-            }
+            for (int k = 0; k < D / 4; k += 2) *reinterpret_cast<float4*>(dst + wg * (D / 2) + 2 * k) = make_float4(o[k].x * f, o[k].y * f, o[k + 1].x * f, o[k + 1].y * f);
             if (wg == 0) {
-                if (P.nsplit > 1) P.part_ml[part] = make_float2(M, L);
-                else if (P.final_ml) P.final_ml[(static_cast<size_t>(s) * P.kv_heads + kvh) * P.rows + row] = make_float2(M, L);
+                if (P.nsplit > 1) P.part_ml[part] = make_float2(m, L);
+                else if (P.final_ml) P.final_ml[(static_cast<size_t>(s) * P.kv_heads + kvh) * P.rows + row] = make_float2(m, L);
             }
         }
     }
@@ -710,11 +701,9 @@ inline bool cache_map(CUtensorMap* map, const uint8_t* base, const AttnP& P, int
 template <int D, int FMT>
 int attn_launch_tc(const AttnP& P, bool general, cudaStream_t st) {
     if constexpr (D == 64 || D == 128) {
-        using C = TcCfg<D, FMT, true>;
-        using N = TcCfg<D, FMT, false>;
-        const int slots = general ? C::KT : N::KT;
+        using C = TcCfg<D, FMT>;
         CUtensorMap mk{}, mv{};
-        if (FMT == 16 && !(cache_map(&mk, P.k, P, D, P.k_row, P.k_head, P.k_seq, slots) && cache_map(&mv, P.v, P, D, P.v_row, P.v_head, P.v_seq, slots)))
+        if (FMT == 16 && !(cache_map(&mk, P.k, P, D, P.k_row, P.k_head, P.k_seq, C::KT) && cache_map(&mv, P.v, P, D, P.v_row, P.v_head, P.v_seq, C::KT)))
             return KCB_UNSUPPORTED_OPERATION;
         static PerDeviceFlag raised[2];
         const dim3 grid(P.row_tiles * P.nsplit, P.kv_heads, P.n_seqs);
@@ -722,8 +711,8 @@ int attn_launch_tc(const AttnP& P, bool general, cudaStream_t st) {
             if (!raise_dynamic_smem(attn_tc_kernel<D, FMT, true>, C::kSmem, raised[0])) return KCB_LAUNCH_FAILURE;
             attn_tc_kernel<D, FMT, true><<<grid, C::kThreads, C::kSmem, st>>>(P, mk, mv);
         } else {
-            if (!raise_dynamic_smem(attn_tc_kernel<D, FMT, false>, N::kSmem, raised[1])) return KCB_LAUNCH_FAILURE;
-            attn_tc_kernel<D, FMT, false><<<grid, N::kThreads, N::kSmem, st>>>(P, mk, mv);
+            if (!raise_dynamic_smem(attn_tc_kernel<D, FMT, false>, C::kSmem, raised[1])) return KCB_LAUNCH_FAILURE;
+            attn_tc_kernel<D, FMT, false><<<grid, C::kThreads, C::kSmem, st>>>(P, mk, mv);
         }
         return launch_status();
     }
