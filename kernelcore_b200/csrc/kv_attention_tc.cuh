@@ -34,7 +34,9 @@ template <int D, int FMT>
 struct TcCfg {
     static constexpr int HK = FMT == 16 ? 64 : 32;             // keys of a tile per softmax warpgroup
     static constexpr int KT = 2 * HK, kRows = 128;
-    static constexpr int kThreads = FMT == 16 ? 384 : 512, kMmaWarp = kThreads / 32 - 1, kProducers = kThreads - 256 - 32;
+    // fp16: three producer warps and the products' warp make the third warpgroup; 4 bits: two producer warpgroups, and one that holds
+    // the products' warp (and three idle ones)
+    static constexpr int kProducers = FMT == 16 ? 96 : 256, kThreads = FMT == 16 ? 384 : 640, kMmaWarp = FMT == 16 ? 11 : 16;
     static constexpr int kPlane = KT * D * 2;                  // one fp16 tile: D / 64 atoms of KT keys x 128 bytes
     static constexpr int kSlot = (FMT == 16 ? 1 : 2) * kPlane; // keys or values of a tile (4 bits: hi, lo)
     static constexpr int kStages = kSlot > 16384 ? 2 : 4;      // of keys, and of values
@@ -47,8 +49,11 @@ struct TcCfg {
     static constexpr int kTile0 = kBars + 256;                 // bitmap of tiles
     static constexpr int kSmem = kTile0 + kDocBits / 8 + 1024; // + room to align the base to 1024 bytes
     static constexpr uint32_t kS = 0, kP = KT, kO = 3 * KT;    // TMEM columns: scores, two buffers of probabilities, outputs
-    static constexpr int kRegsSoftmax = FMT == 16 ? 224 : 184, kRegsProducer = FMT == 16 ? 56 : 72, kRegsLaunch = FMT == 16 ? 168 : 128;
-    static_assert(2 * 128 * kRegsSoftmax + (kThreads - 256) * kRegsProducer <= kThreads * kRegsLaunch, "the softmax warpgroups take what the producers give up");
+    // registers per thread: what a launch of kThreads gets (checked when the kernel is first launched: with fewer, the softmax
+    // warpgroups would wait for ever for registers that nobody gives up), and after the hand-over
+    static constexpr int kRegsLaunch = FMT == 16 ? 168 : 96, kRegsSoftmax = FMT == 16 ? 224 : 152, kRegsProducer = FMT == 16 ? 56 : 64, kRegsMma = 40;
+    static_assert(2 * 128 * kRegsSoftmax + (FMT == 16 ? 128 * kRegsProducer : 256 * kRegsProducer + 128 * kRegsMma) <= kThreads * kRegsLaunch,
+                  "the softmax warpgroups take what the others give up");
     static_assert(kO + D <= 512 && kMetaBytes % 16 == 0 && kSmem <= kMaxSmem && kSmem > kMaxSmem / 2, "TMEM columns; one CTA per SM");
 };
 
@@ -150,33 +155,40 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
-// Capped scores: y = tanh(u) cap, u = y on entry.  The power series below 0.55 (see tanh_series), elsewhere 1 - 2 / (e^2|u| + 1): there
-// the difference costs one bit.  A warp whose scores are all small against the cap, as most are, takes the series alone.
+// Capped scores: y = tanh(y c), c positive; the cap itself is multiplied later.  A power series for |u| < 0.3 (to u^9: 5e-8) or
+// 0.55 (to u^15, see tanh_series), elsewhere 1 - 2 / (e^2|u| + 1): there the difference costs one bit.  A warp takes the shortest
+// that holds for all its scores, most of which are small against the cap.
 template <int H>
-__device__ __forceinline__ void cap_scores(float (&y)[H][32], float cap) {
-    float big = 0.0f;
+__device__ __forceinline__ void cap_scores(float (&y)[H][32], float c) {
+    float hi = y[0][0], lo = y[0][0];
 #pragma unroll
     for (int h = 0; h < H; ++h)
 #pragma unroll
-        for (int k = 0; k < 32; ++k) big = fmaxf(big, fabsf(y[h][k]));
-    const bool small = __all_sync(0xffffffffu, big < 0.55f);
+        for (int k = 0; k < 32; k += 2) hi = max3(hi, y[h][k], y[h][k + 1]), lo = -max3(-lo, -y[h][k], -y[h][k + 1]);
+    const float big = fmaxf(hi, -lo) * c;
+    const bool tiny = __all_sync(0xffffffffu, big < 0.3f), small = __all_sync(0xffffffffu, big < 0.55f);
+    if (tiny) {
 #pragma unroll
-    for (int h = 0; h < H; ++h)
+        for (int h = 0; h < H; ++h)
 #pragma unroll
-        for (int k = 0; k < 32; k += 2) {
-            const float2 u = make_float2(y[h][k], y[h][k + 1]), w = mul2(u, u);
-            float2 r = fma2(both(-1.4558344e-3f), w, both(3.5921280e-3f));
-            r = fma2(r, w, both(-8.8632355e-3f));
-            r = fma2(r, w, both(2.1869488e-2f));
-            r = fma2(r, w, both(-5.3968254e-2f));
-            r = fma2(r, w, both(1.3333333e-1f));
-            r = fma2(r, w, both(-3.3333333e-1f));
-            r = mul2(fma2(mul2(u, w), r, u), both(cap));
-            if (!small) {
-                if (fabsf(u.x) >= 0.55f) r.x = copysignf(cap - __fdividef(2.0f * cap, ex2(2.0f * kLog2e * fabsf(u.x)) + 1.0f), u.x);
-                if (fabsf(u.y) >= 0.55f) r.y = copysignf(cap - __fdividef(2.0f * cap, ex2(2.0f * kLog2e * fabsf(u.y)) + 1.0f), u.y);
+            for (int k = 0; k < 32; k += 2) {
+                const float2 u = mul2(make_float2(y[h][k], y[h][k + 1]), both(c)), w = mul2(u, u);
+                float2 r = fma2(both(2.1869488e-2f), w, both(-5.3968254e-2f));
+                r = fma2(r, w, both(1.3333333e-1f));
+                r = fma2(r, w, both(-3.3333333e-1f));
+                r = fma2(mul2(u, w), r, u);
+                y[h][k] = r.x, y[h][k + 1] = r.y;
             }
-            y[h][k] = r.x, y[h][k + 1] = r.y;
+        return;
+    }
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+            const float u = y[h][k] * c;
+            float r = tanh_series(u);
+            if (!small && fabsf(u) >= 0.55f) r = copysignf(1.0f - __fdividef(2.0f, ex2(2.0f * kLog2e * fabsf(u)) + 1.0f), u);
+            y[h][k] = r;
         }
 }
 
@@ -272,7 +284,8 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
     // (after an expired wait every loop below runs on, without products, so that every barrier finds its arrivals)
 
     if (wg >= 2) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsProducer));
+        if (FMT == 16 || wg < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsProducer));
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsMma));
         if (warp == C::kMmaWarp) {
             // ---- products ----------------------------------------------------------------------------------------------------
             int i = 0;  // tiles so far, over both passes: stages and parities go by it
@@ -331,50 +344,59 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
                 __syncwarp();
                 if (FMT != 16 || !__syncthreads_or(0) || careful) break;
             }
-        } else {
+        } else if (warp < C::kMmaWarp) {
             // ---- producers ---------------------------------------------------------------------------------------------------
             const int ptid = tid - 256;
-            auto unpack = [&](const uint8_t* src, bool value, uint8_t* dst, int t0) {  // 4 bits: values as hi and lo tiles
+            // 4 bits: a thread has group c of row r of every tile: the pieces (b, c) of 8 channels of every block b (values: groups 2 c
+            // and 2 c + 1).  Its bytes are requested while it unpacks something else.
+            struct Raw {
+                unsigned v[NB], par[NB];
+            };
+            const int ur = ptid >> 2, uc = ptid & 3;
+            auto request = [&](Raw& w, const uint8_t* src, int tile) {
+                const int t = begin + tile * KT + ur;
+                const bool ok = tile < nt && t < end;  // a row behind those in use is zeros
                 const uint8_t* b0 = src + static_cast<size_t>(s) * P.seq_bytes;
-                // an item is group c of a row: the pieces (b, c) of 8 channels of every block b (values: groups 2 c and 2 c + 1)
-#pragma unroll 1
-                for (int x = ptid; x < KT * 4; x += C::kProducers) {
-                    const int r = x >> 2, c = x & 3;
-                    const bool ok = t0 + r < end;
-                    const size_t at = static_cast<size_t>(kvh) * P.cap + (ok ? t0 + r : 0);
-                    const uint8_t* rowp = b0 + at * (D / 2);
-                    const unsigned* par = reinterpret_cast<const unsigned*>(b0 + P.par_off + at * (4 * NB));
-                    unsigned pw[NB], v[NB];
-                    if constexpr (NB == 4) {
-                        const uint4 t = *reinterpret_cast<const uint4*>(rowp + c * 16), q = *reinterpret_cast<const uint4*>(par);
-                        v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
-                        pw[0] = q.x, pw[1] = q.y, pw[2] = q.z, pw[3] = q.w;
-                    } else {
-                        const uint2 t = *reinterpret_cast<const uint2*>(rowp + c * 8), q = *reinterpret_cast<const uint2*>(par);
-                        v[0] = t.x, v[1] = t.y;
-                        pw[0] = q.x, pw[1] = q.y;
-                    }
+                const size_t at = static_cast<size_t>(kvh) * P.cap + (ok ? t : 0);
+                const uint8_t* rowp = b0 + at * (D / 2) + uc * (4 * NB);
+                const uint8_t* par = b0 + P.par_off + at * (4 * NB);
+                if constexpr (NB == 4) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(rowp), q = *reinterpret_cast<const uint4*>(par);
+                    w.v[0] = x.x, w.v[1] = x.y, w.v[2] = x.z, w.v[3] = x.w;
+                    w.par[0] = q.x, w.par[1] = q.y, w.par[2] = q.z, w.par[3] = q.w;
+                } else {
+                    const uint2 x = *reinterpret_cast<const uint2*>(rowp), q = *reinterpret_cast<const uint2*>(par);
+                    w.v[0] = x.x, w.v[1] = x.y;
+                    w.par[0] = q.x, w.par[1] = q.y;
+                }
+                if (!ok)
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        // a row behind those in use is zeros, and a hidden slot's scales may be anything
-                        if (!ok || not_finite2(pw[b])) pw[b] = 0u;
-                        const unsigned w = value ? __byte_perm(v[b / 2], v[NB / 2 + b / 2], b & 1 ? 0x7632 : 0x5410) : v[b];
-                        const float2 dm = __half22float2(*reinterpret_cast<__half2*>(&pw[b]));
-                        // codes about their middle, 2^23 + code less 2^23 + 8: no integer conversion
-                        const float2 d = both(dm.x), mid = both(fmaf(8.0f, dm.x, dm.y));
-                        unsigned hi[4], lo[4];
+                    for (int b = 0; b < NB; ++b) w.par[b] = 0u;
+            };
+            auto unpack = [&](const Raw& raw, bool value, uint8_t* dst) {  // values as hi and lo tiles
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const float2 code = add2(make_float2(__uint_as_float(0x4B000000u | (w >> (8 * k) & 15u)), __uint_as_float(0x4B000000u | (w >> (8 * k + 4) & 15u))), both(-8388616.0f));
-                            const float2 x2 = fma2(d, code, mid);
-                            const __half2 h = __floats2half2_rn(fminf(x2.x, 65504.0f), fminf(x2.y, 65504.0f));  // the rest of a larger value goes to lo
-                            const float2 f = __half22float2(h);
-                            hi[k] = h2_bits(h), lo[k] = h2_bits(__floats2half2_rn(x2.x - f.x, x2.y - f.y));
-                        }
-                        uint8_t* o = dst + swz(KT, r, 4 * b + c);
-                        *reinterpret_cast<uint4*>(o) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                        *reinterpret_cast<uint4*>(o + C::kPlane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                for (int b = 0; b < NB; ++b) {
+                    const unsigned pw = not_finite2(raw.par[b]) ? 0u : raw.par[b];  // (a hidden slot's scales may be anything)
+                    const unsigned w = value ? __byte_perm(raw.v[b / 2], raw.v[NB / 2 + b / 2], b & 1 ? 0x7632 : 0x5410) : raw.v[b];
+                    const float d = half_bits_to_float(pw & 0xFFFFu), m = half_bits_to_float(pw >> 16);
+                    const float2 mid = both(fmaf(8.0f, d, m));
+                    // codes about their middle without an integer conversion: the bits of 2^23 + code, less 2^23 + 8
+                    const unsigned even = w & 0x0F0F0F0Fu, odd = (w >> 4) & 0x0F0F0F0Fu;
+                    const bool large = fmaf(15.0f, d, fabsf(m)) > 65504.0f;  // the format reaches a little further than fp16
+                    unsigned hi[4], lo[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float2 code = add2(make_float2(__uint_as_float(__byte_perm(even, 0x4B000000u, 0x7440 + k)), __uint_as_float(__byte_perm(odd, 0x4B000000u, 0x7440 + k))),
+                                                 both(-8388616.0f));
+                        const float2 x = fma2(both(d), code, mid);
+                        __half2 h = __floats2half2_rn(x.x, x.y);
+                        if (large) h = __floats2half2_rn(fminf(x.x, 65504.0f), fminf(x.y, 65504.0f));  // the rest goes to lo
+                        const float2 l = fma2(__half22float2(h), both(-1.0f), x);
+                        hi[k] = h2_bits(h), lo[k] = h2_bits(__floats2half2_rn(l.x, l.y));
                     }
+                    uint8_t* o = dst + swz(KT, ur, 4 * b + uc);
+                    *reinterpret_cast<uint4*>(o) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4*>(o + C::kPlane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
             };
             auto beside = [&](int t0, int st, int first, int threads) {  // positions and documents of a tile's slots
@@ -387,17 +409,23 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
             const bool beside_wanted = GEN && (P.positions || P.k_doc);
             int i = 0;
             if constexpr (FMT != 16) {
-                for (int tile = next(-1); tile < nt; tile = next(tile), ++i) {
-                    const int st = i % C::kStages, ph = (i / C::kStages - 1) & 1, t0 = begin + tile * KT;
+                Raw rk, rv;
+                int tile = next(-1);
+                request(rk, P.k, tile);
+                for (; tile < nt; ++i) {
+                    const int st = i % C::kStages, ph = (i / C::kStages - 1) & 1, t0 = begin + tile * KT, after = next(tile);
+                    request(rv, P.v, tile);
                     if (i >= C::kStages) tc_wait(&kempty[st], ph, fail);
-                    unpack(P.k, false, sm + C::kOffK + st * C::kSlot, t0);
+                    unpack(rk, false, sm + C::kOffK + st * C::kSlot);
                     fence_async_shared();
                     bar_arrive(&kfull[st]);
+                    request(rk, P.k, after);
                     if (i >= C::kStages) tc_wait(&vempty[st], ph, fail);
-                    unpack(P.v, true, sm + C::kOffV + st * C::kSlot, t0);
+                    unpack(rv, true, sm + C::kOffV + st * C::kSlot);
                     if (beside_wanted) beside(t0, st, ptid, C::kProducers);
                     fence_async_shared();
                     bar_arrive(&vfull[st]);
+                    tile = after;
                 }
             } else {
                 for (bool careful = false;; careful = true) {
@@ -490,13 +518,20 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
 #define Y(k) yy[(k) >> 5][(k) & 31]
             tc_before_sync();
             bar_arrive(sread);
+            float fac = ysc;  // what turns y into base-2 scores
             if (GEN) {
-#pragma unroll
-                for (int k = 0; k < HK; k += 2) {
-                    const float2 t = mul2(make_float2(Y(k), Y(k + 1)), both(ysc));
-                    Y(k) = t.x, Y(k + 1) = t.y;
+                if (P.cap_out != 0.0f) {
+                    cap_scores(yy, ysc);
+                    fac = P.cap_out;
                 }
-                if (P.cap_out != 0.0f) cap_scores(yy, P.cap_out);
+                if (P.mask || P.bias_step != 0.0f) {
+#pragma unroll
+                    for (int k = 0; k < HK; k += 2) {
+                        const float2 t = mul2(make_float2(Y(k), Y(k + 1)), both(fac));
+                        Y(k) = t.x, Y(k + 1) = t.y;
+                    }
+                    fac = 1.0f;
+                }
                 if (P.positions || P.k_doc) tc_wait(FMT == 16 ? &mfull[st] : &vfull[st], (i / C::kStages) & 1, fail);
                 if (P.mask) {
                     const unsigned short* mp = ri.mask + t0;
@@ -528,8 +563,14 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
                         for (int k = 0; k < HK; ++k) Y(k) -= ri.slope * fabsf(qp - static_cast<float>(meta[k]));
                     } else {
                         const float far = static_cast<float>(ri.pos) - static_cast<float>(t0);
+                        if (__all_sync(0xffffffffu, far >= static_cast<float>(HK - 1))) {  // all of them in front of the query: no absolute value
+                            const float nearest = ri.slope * (static_cast<float>(HK - 1) - far);
 #pragma unroll
-                        for (int k = 0; k < HK; ++k) Y(k) -= ri.slope * fabsf(far - static_cast<float>(k));
+                            for (int k = 0; k < HK; ++k) Y(k) += fmaf(ri.slope, static_cast<float>(k - (HK - 1)), nearest);
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < HK; ++k) Y(k) -= ri.slope * fabsf(far - static_cast<float>(k));
+                        }
                     }
                 }
                 if (P.causal && P.positions) {
@@ -564,7 +605,7 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
                 mx = max3(mx, Y(k), Y(k + 1));
                 if (k + 2 < HK) mx1 = max3(mx1, Y(k + 2), Y(k + 3));
             }
-            mx = fmaxf(mx, mx1) * (GEN ? 1.0f : ysc);
+            mx = fmaxf(mx, mx1) * fac;
             maxima[((i & 1) * 2 + wg) * C::kRows + r] = mx;
             bar_arrive(mxfull);
             tc_wait(mxfull, i & 1, fail);
@@ -580,7 +621,7 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
                 unsigned hi[16], lo[16];
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
-                    const float2 v = make_float2(yy[h][2 * k], yy[h][2 * k + 1]), e = GEN ? add2(v, ref) : fma2(v, both(ysc), ref);
+                    const float2 v = make_float2(yy[h][2 * k], yy[h][2 * k + 1]), e = fma2(v, both(fac), ref);
                     const float2 p = make_float2(ex2(e.x), ex2(e.y));
                     if (k & 1) sum1 = add2(sum1, p);
                     else sum = add2(sum, p);
@@ -698,6 +739,16 @@ inline bool cache_map(CUtensorMap* map, const uint8_t* base, const AttnP& P, int
     return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<uint8_t*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+// Once per device: room for dynamic shared memory, and whether the kernel was built with the registers that its hand-over counts on.
+template <class Kern>
+inline bool prepare_kernel(Kern kern, int smem, int regs, PerDeviceFlag& f) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return false;
+    if (f.set[dev].load(std::memory_order_acquire)) return true;
+    cudaFuncAttributes a;
+    if (cudaFuncGetAttributes(&a, kern) != cudaSuccess || a.numRegs < regs) return false;
+    return raise_dynamic_smem(kern, smem, f);
+}
 template <int D, int FMT>
 int attn_launch_tc(const AttnP& P, bool general, cudaStream_t st) {
     if constexpr (D == 64 || D == 128) {
@@ -708,10 +759,10 @@ int attn_launch_tc(const AttnP& P, bool general, cudaStream_t st) {
         static PerDeviceFlag raised[2];
         const dim3 grid(P.row_tiles * P.nsplit, P.kv_heads, P.n_seqs);
         if (general) {
-            if (!raise_dynamic_smem(attn_tc_kernel<D, FMT, true>, C::kSmem, raised[0])) return KCB_LAUNCH_FAILURE;
+            if (!prepare_kernel(attn_tc_kernel<D, FMT, true>, C::kSmem, C::kRegsLaunch, raised[0])) return KCB_LAUNCH_FAILURE;
             attn_tc_kernel<D, FMT, true><<<grid, C::kThreads, C::kSmem, st>>>(P, mk, mv);
         } else {
-            if (!raise_dynamic_smem(attn_tc_kernel<D, FMT, false>, C::kSmem, raised[1])) return KCB_LAUNCH_FAILURE;
+            if (!prepare_kernel(attn_tc_kernel<D, FMT, false>, C::kSmem, C::kRegsLaunch, raised[1])) return KCB_LAUNCH_FAILURE;
             attn_tc_kernel<D, FMT, false><<<grid, C::kThreads, C::kSmem, st>>>(P, mk, mv);
         }
         return launch_status();
