@@ -117,13 +117,30 @@ __device__ __forceinline__ unsigned code_pair(unsigned w) {
     else asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(n), "r"(SHIFT ? 0x64006400u : 0x74007400u));
     return r;
 }
+// Packed fp32 pairs (one instruction for two values, each rounded as the scalar operation).
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)), "l"(reinterpret_cast<unsigned long long&>(c)));
+    return reinterpret_cast<float2&>(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+    return reinterpret_cast<float2&>(r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+    return reinterpret_cast<float2&>(r);
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 __device__ __forceinline__ unsigned h2_bits(__half2 h) { return *reinterpret_cast<unsigned*>(&h); }
 // (x, y) = hi + lo, each a pair of fp16 numbers: hi rounds to nearest, lo holds the next 11 bits
 __device__ __forceinline__ void split2(float x, float y, unsigned& hi, unsigned& lo) {
     const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
+    const float2 l = fma2(__half22float2(h), both(-1.0f), make_float2(x, y));
     hi = h2_bits(h);
-    lo = h2_bits(__floats2half2_rn(x - f.x, y - f.y));
+    lo = h2_bits(__floats2half2_rn(l.x, l.y));
 }
 // Power of two that brings |x| near 2^11, and its inverse; 1 for zero, infinite and NaN rows as far as their exponents allow.
 __device__ __forceinline__ void row_scale(float amax, float& up, float& down) {
@@ -332,6 +349,32 @@ __device__ __forceinline__ void load_tile(const AttnP& P, const uint8_t* base, l
     }
 }
 
+// The same for a tile of ROWS slots that are all in use, by one warp: no predicates, and where an address moves on by constants only
+// the copies.  (4-bit parameters of narrow heads are not aligned to 16 bytes: those take the form above.)
+__device__ __forceinline__ void cp16_all(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+template <int D, int FMT, int ROWS>
+__device__ __forceinline__ void load_tile_full(const uint8_t* codes_or_rows, const uint8_t* params, long long row, int t0, uint32_t dst, int lane) {
+    using T = Tile<D, FMT>;
+    if constexpr (FMT == 16) {
+        const __half* src = reinterpret_cast<const __half*>(codes_or_rows);
+        constexpr int kChunks = D / 8;
+#pragma unroll
+        for (int i = 0; i < ROWS * kChunks / 32; ++i) {
+            const int x = i * 32 + lane, r = x / kChunks, ch = x % kChunks;
+            cp16_all(dst + r * T::kRow + ch * 16, src + static_cast<long long>(t0 + r) * row + ch * 8);
+        }
+    } else {
+        const uint8_t* src = codes_or_rows + static_cast<size_t>(t0) * (D / 2) + lane * 16;
+#pragma unroll
+        for (int i = 0; i < ROWS * (D / 32) / 32; ++i) cp16_all(dst + (i * 32 + lane) * 16, src + i * 512);
+        if constexpr (T::NB % 4 == 0) {
+            const uint8_t* par = params + static_cast<size_t>(t0) * T::kPar + lane * 16;
+#pragma unroll
+            for (int i = 0; i < ROWS * T::kPar / 512; ++i) cp16_all(dst + ROWS * T::kRow + (i * 32 + lane) * 16, par + i * 512);
+        }
+    }
+}
+
 // NW 32-bit words at a 4-byte (or wider, as NW allows) aligned shared address
 template <int NW>
 __device__ __forceinline__ void lds_words(unsigned (&w)[NW], const uint8_t* p) {
@@ -392,24 +435,28 @@ template <int FMT>
 constexpr float kCodeUp = FMT == 16 ? 1.0f : 1024.0f;
 
 // ---- rows kernel: up to eight rows per CTA, many keys ---------------------------------------------------------------------
-// For single tokens.  What bounds it is reading the cache once.  Each of the CTA's four warps works alone on 16-slot blocks
-// (its own copies in flight, its own running maximum), so nothing waits for a neighbour; the eight rows' hi and lo halves are
-// stacked into one 16-row fragment, which makes the second half of the precision free of extra products.
+// For single tokens.  What bounds it is reading the cache once.  Each of the CTA's four warps works alone on blocks of slots (its own
+// copies in flight, its own running maximum), so nothing waits for a neighbour; the eight rows' hi and lo halves are stacked
+// into one 16-row fragment, which makes the second half of the precision free of extra products.  16 slots a block for fp16 (whose
+// ring then fills the shared memory with eight warps), 32 for 4 bits.
+// MODE 0: scores as they are; 1: with a cap or a distance bias, slot = position; 2: positions, documents or an additive mask too.
+// In the first two a row sees the slots below a limit.
 constexpr int kRowsWarps = 4;
 template <int D, int FMT>
 struct RowsCfg {
-    static constexpr int kBlock = 2 * Tile<D, FMT>::bytes(16);
-    static constexpr int kStages = FMT == 16 ? (D >= 128 ? 3 : 4) : 6;
+    static constexpr int kSlots = FMT == 16 ? 16 : 32;
+    static constexpr int kBlock = 2 * Tile<D, FMT>::bytes(kSlots);
+    static constexpr int kStages = FMT == 16 && D < 128 ? 4 : 3;
     static constexpr int kMerge = kRowsWarps * 8 * (D + 4) * 4;
     static constexpr int kRing = kRowsWarps * kStages * kBlock;
     static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
 };
 
-template <int D, int FMT, bool GEN>
-__global__ void __launch_bounds__(32 * kRowsWarps) attn_rows_kernel(const __grid_constant__ AttnP P) {
+template <int D, int FMT, int MODE>
+__global__ void __launch_bounds__(32 * kRowsWarps, FMT == 16 && D == 128 ? 2 : 1) attn_rows_kernel(const __grid_constant__ AttnP P) {
     using C = RowsCfg<D, FMT>;
     using T = Tile<D, FMT>;
-    constexpr int NB = D / 32, KS = D / 16, NT = D / 8;
+    constexpr int NB = D / 32, KS = D / 16, NT = D / 8, SL = C::kSlots, U = SL / 16;
     extern __shared__ __align__(16) uint8_t sm[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
     const int split = blockIdx.x, kvh = blockIdx.y / P.row_tiles, row0 = (blockIdx.y % P.row_tiles) * 8, s = blockIdx.z;
@@ -423,18 +470,33 @@ __global__ void __launch_bounds__(32 * kRowsWarps) attn_rows_kernel(const __grid
 
     uint8_t* ring = sm + warp * C::kStages * C::kBlock;
     const uint32_t ring_a = smem_u32(ring);
-    const int nblk = max(0, (end - begin + 15) / 16), mine = nblk > warp ? (nblk - warp + kRowsWarps - 1) / kRowsWarps : 0;
-    auto fetch = [&](int i) {
+    const int nblk = (end - begin + SL - 1) / SL, mine = nblk > warp ? (nblk - warp + kRowsWarps - 1) / kRowsWarps : 0;
+    const uint8_t *kb, *vb, *kpar = nullptr, *vpar = nullptr;  // this sequence's and head's rows
+    if (FMT == 16) {
+        kb = P.k + 2 * (static_cast<size_t>(s) * P.k_seq + static_cast<size_t>(kvh) * P.k_head);
+        vb = P.v + 2 * (static_cast<size_t>(s) * P.v_seq + static_cast<size_t>(kvh) * P.v_head);
+    } else {
+        const size_t seq = static_cast<size_t>(s) * P.seq_bytes, at = static_cast<size_t>(kvh) * P.cap;
+        kb = P.k + seq + at * (D / 2), vb = P.v + seq + at * (D / 2);
+        kpar = P.k + seq + P.par_off + at * T::kPar, vpar = P.v + seq + P.par_off + at * T::kPar;
+    }
+    constexpr bool kWhole = FMT == 16 ? (SL * D / 8) % 32 == 0 : NB % 4 == 0;
+    auto fetch = [&](int i, int stage) {
         if (i < mine) {
-            const int t0 = begin + (warp + i * kRowsWarps) * 16;
-            const uint32_t dst = ring_a + (i % C::kStages) * C::kBlock;
-            load_tile<D, FMT, 16, 32>(P, P.k, P.k_row, P.k_head, P.k_seq, s, kvh, t0, end, dst, lane);
-            load_tile<D, FMT, 16, 32>(P, P.v, P.v_row, P.v_head, P.v_seq, s, kvh, t0, end, dst + T::bytes(16), lane);
+            const int t0 = begin + (warp + i * kRowsWarps) * SL;
+            const uint32_t dst = ring_a + stage * C::kBlock;
+            if (kWhole && t0 + SL <= end) {
+                load_tile_full<D, FMT, SL>(kb, kpar, P.k_row, t0, dst, lane);
+                load_tile_full<D, FMT, SL>(vb, vpar, P.v_row, t0, dst + T::bytes(SL), lane);
+            } else {
+                load_tile<D, FMT, SL, 32>(P, P.k, P.k_row, P.k_head, P.k_seq, s, kvh, t0, end, dst, lane);
+                load_tile<D, FMT, SL, 32>(P, P.v, P.v_row, P.v_head, P.v_seq, s, kvh, t0, end, dst + T::bytes(SL), lane);
+            }
         }
         cp_commit();
     };
 #pragma unroll
-    for (int i = 0; i < C::kStages - 1; ++i) fetch(i);
+    for (int i = 0; i < C::kStages - 1; ++i) fetch(i, i);
 
     // the row's query as hi (registers 0, 2) and lo (1, 3) fragments, scaled; block sums for the minima
     unsigned qf[KS][4];
@@ -469,106 +531,111 @@ __global__ void __launch_bounds__(32 * kRowsWarps) attn_rows_kernel(const __grid
         }
     }
     const float ysc = P.sc * down * kCodeUp<FMT>;
-    RowInfo ri;
-    int limit = n, prefix = 0;
-    if (GEN) {
-        ri = row_info(P, s, kvh, n, row);
-        prefix = P.prefix ? P.prefix[s] : 0;
-    } else {
-        if (P.causal) limit = min(n, row_pos(P, s, n, token) + 1);
-        if (!valid) limit = 0;
-    }
+    RowInfo ri{};
+    int limit = valid ? end : 0;
+    const int prefix = P.prefix ? P.prefix[s] : 0;
+    if (MODE) ri = row_info(P, s, kvh, n, row);
+    if (MODE < 2 && P.causal && valid) limit = min(end, max(prefix, row_pos(P, s, n, token) + 1));
+    const bool hides = MODE == 2 || (P.causal && (P.n_tokens > 1 || P.next_pos || P.q_pos));  // slots in use may be hidden from a row
+    const float rpos = static_cast<float>(ri.pos);
 
-    float o[NT][4], om[FMT == 16 ? 1 : NB], m = -INFINITY, l = 0.0f;
+    float o[NT][4], m = -INFINITY, l = 0.0f;
+    float2 om[FMT == 16 ? 1 : NB];
 #pragma unroll
     for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
 #pragma unroll
-    for (int b = 0; b < (FMT == 16 ? 1 : NB); ++b) om[b] = 0.0f;
+    for (int b = 0; b < (FMT == 16 ? 1 : NB); ++b) om[b] = make_float2(0.0f, 0.0f);
 
+    int stage = 0;
     for (int i = 0; i < mine; ++i) {
         cp_wait<C::kStages - 2>();
         __syncwarp();
-        fetch(i + C::kStages - 1);  // into the stage that was read in the last round
-        const uint8_t* kt = ring + (i % C::kStages) * C::kBlock;
-        const uint8_t* vt = kt + T::bytes(16);
-        const int t0 = begin + (warp + i * kRowsWarps) * 16;
-        float y[4];
+        fetch(i + C::kStages - 1, stage == 0 ? C::kStages - 1 : stage - 1);  // into the stage that was read in the last round
+        const uint8_t* kt = ring + stage * C::kBlock;
+        const uint8_t* vt = kt + T::bytes(SL);
+        if (++stage == C::kStages) stage = 0;
+        const int t0 = begin + (warp + i * kRowsWarps) * SL;
+        float y[U][4];
         if (FMT == 16) {
             float sc[2][4] = {};
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int k2 = 0; k2 < KS / 2; ++k2)
 #pragma unroll
-                for (int k2 = 0; k2 < KS / 2; ++k2) {
+                for (int t = 0; t < 2; ++t) {
                     unsigned b[4];
                     ldsm4(b, smem_u32(kt) + (t * 8 + (lane & 7)) * T::kRow + k2 * 64 + (lane >> 3) * 16);
                     mma16816(sc[t], qf[2 * k2], b[0], b[1]);
                     mma16816(sc[t], qf[2 * k2 + 1], b[2], b[3]);
                 }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = sc[j >> 1][j & 1] + sc[j >> 1][2 + (j & 1)];
+            for (int j = 0; j < 4; ++j) y[0][j] = sc[j >> 1][j & 1] + sc[j >> 1][2 + (j & 1)];
         } else {
-            const uint8_t* kp = kt + 16 * T::kRow;
+            const uint8_t* kp = kt + SL * T::kRow;
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                unsigned w[NB], p0[NB], p1[NB];
-                lds_words(w, kt + row_of_column<FMT>(t, g) * T::kRow + c * 4 * NB);
-                lds_words(p0, kp + (t * 8 + c) * T::kPar);
-                lds_words(p1, kp + (t * 8 + c + 4) * T::kPar);
-                float y0 = 0.0f, y1 = 0.0f;
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    const unsigned hi = w[b] >> 8;
-                    mma16816(a, qf[2 * b], code_pair<false, false>(w[b]), code_pair<true, false>(w[b]));
-                    mma16816(a, qf[2 * b + 1], code_pair<false, false>(hi), code_pair<true, false>(hi));
-                    const float2 d0 = __half22float2(*reinterpret_cast<__half2*>(&p0[b])), d1 = __half22float2(*reinterpret_cast<__half2*>(&p1[b]));
-                    y0 = fmaf(d0.x, a[0] + a[2], fmaf(d0.y, qs[b], y0));
-                    y1 = fmaf(d1.x, a[1] + a[3], fmaf(d1.y, qs[b], y1));
+                for (int t = 0; t < 2; ++t) {
+                    unsigned w[NB], p0[NB], p1[NB];
+                    lds_words(w, kt + (u * 16 + row_of_column<FMT>(t, g)) * T::kRow + c * 4 * NB);
+                    lds_words(p0, kp + (u * 16 + t * 8 + c) * T::kPar);
+                    lds_words(p1, kp + (u * 16 + t * 8 + c + 4) * T::kPar);
+                    float2 acc = make_float2(0.0f, 0.0f);
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        const unsigned hi = w[b] >> 8;
+                        mma16816(a, qf[2 * b], code_pair<false, false>(w[b]), code_pair<true, false>(w[b]));
+                        mma16816(a, qf[2 * b + 1], code_pair<false, false>(hi), code_pair<true, false>(hi));
+                        const float2 d0 = __half22float2(*reinterpret_cast<__half2*>(&p0[b])), d1 = __half22float2(*reinterpret_cast<__half2*>(&p1[b]));
+                        acc = fma2(make_float2(d0.x, d1.x), add2(make_float2(a[0], a[1]), make_float2(a[2], a[3])), fma2(make_float2(d0.y, d1.y), both(qs[b]), acc));
+                    }
+                    y[u][2 * t] = acc.x, y[u][2 * t + 1] = acc.y;
                 }
-                y[2 * t] = y0, y[2 * t + 1] = y1;
-            }
         }
         float mx = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int t = t0 + slot_of<FMT>(c, j);
-            if (GEN) {
-                const KeyInfo key = key_info(P, s, kvh, t, end);
-                y[j] = general_score(P, y[j] * ysc, ri, key, t, end, prefix);
-            } else {
-                y[j] = t < min(limit, end) ? y[j] * ysc : -INFINITY;
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int t = t0 + u * 16 + slot_of<FMT>(c, j);
+                float& v = y[u][j];
+                v *= ysc;
+                if (MODE == 2) {
+                    v = general_score(P, v, ri, key_info(P, s, kvh, t, end), t, end, prefix);
+                } else {
+                    if (MODE == 1) {
+                        if (P.cap_out != 0.0f) v = tanh_acc(v) * P.cap_out;
+                        if (P.bias_step != 0.0f) v -= ri.slope * fabsf(rpos - static_cast<float>(t));
+                    }
+                    if (t >= limit) v = -INFINITY;
+                }
+                mx = fmaxf(mx, v);
             }
-            mx = fmaxf(mx, y[j]);
-        }
         if (P.scores && valid) {
             float* sp = P.scores + ((static_cast<size_t>(s) * P.kv_heads + kvh) * P.rows + row) * P.cap + t0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (t0 + slot_of<FMT>(c, j) < end) sp[slot_of<FMT>(c, j)] = y[j];
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (t0 + u * 16 + slot_of<FMT>(c, j) < end) sp[u * 16 + slot_of<FMT>(c, j)] = y[u][j];
         }
-        unsigned vp[4][FMT == 16 ? 1 : NB];
         if (FMT != 16) {
-            const uint8_t* pp = vt + 16 * T::kRow;
-            unsigned big = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                lds_words(vp[j], pp + slot_of<FMT>(c, j) * T::kPar);
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    if (y[j] == -INFINITY) vp[j][b] = 0u;  // a hidden slot's scales may be anything
-                    big |= vp[j][b] & 0x7FFFu;
-                }
-            }
             // p d must stay below fp16's largest number.  With every d below 16 it does; larger scales raise the reference.
             // (The OR is at least the largest d; scales of 2 and more may come here without need, and lose nothing.)
-            if (__any_sync(0xffffffffu, big >= 0x4C00u)) {
+            const uint8_t* pp = vt + SL * T::kRow;
+            unsigned big = 0;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    unsigned dm = 0;
+            for (int x = 0; x < SL * NB / 32; ++x) big |= *reinterpret_cast<const unsigned*>(pp + 4 * (x * 32 + lane));
+            if (__any_sync(0xffffffffu, (big & 0x7FFFu) >= 0x4C00u)) {
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) dm = max(dm, vp[j][b] & 0x7FFFu);
-                    if (y[j] != -INFINITY) mx = fmaxf(mx, y[j] + static_cast<float>(max(0, static_cast<int>(dm >> 10) - 18)));
-                }
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        unsigned dm = 0;
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) dm = max(dm, *reinterpret_cast<const unsigned*>(pp + (u * 16 + slot_of<FMT>(c, j)) * T::kPar + 4 * b) & 0x7FFFu);
+                        if (y[u][j] != -INFINITY) mx = fmaxf(mx, y[u][j] + static_cast<float>(max(0, static_cast<int>(dm >> 10) - 18)));
+                    }
             }
         }
         mx = quad_max(mx);
@@ -580,18 +647,20 @@ __global__ void __launch_bounds__(32 * kRowsWarps) attn_rows_kernel(const __grid
             l *= al;
             if (FMT != 16)
 #pragma unroll
-                for (int b = 0; b < NB; ++b) om[b] *= al;
+                for (int b = 0; b < NB; ++b) om[b].x *= al, om[b].y *= al;
             m = mn;
         }
         const float ref = m == -INFINITY ? 0.0f : m - kPShift;
-        float p[4];
+        float p[U][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            p[j] = ex2(y[j] - ref);
-            l += p[j];
-        }
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                p[u][j] = ex2(y[u][j] - ref);
+                l += p[u][j];
+            }
         if (FMT == 16) {
-            if (GEN || (P.causal && (P.n_tokens > 1 || P.next_pos))) {  // rows may hide slots: an infinity or NaN there must not reach them as 0 * inf
+            if (hides) {  // an infinity or NaN in a hidden slot must not reach the row as 0 * inf
                 bool odd = false;
 #pragma unroll
                 for (int x = 0; x < (16 * D / 8) / 32; ++x) {
@@ -601,7 +670,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps) attn_rows_kernel(const __grid
                 if (__any_sync(0xffffffffu, odd)) {  // rare: such values go to the rows that see them one by one, and become zeros
 #pragma unroll 1
                     for (int t = 0; t < 16; ++t) {
-                        const float pv = (t & 8) ? ((t & 1) ? p[3] : p[2]) : ((t & 1) ? p[1] : p[0]);
+                        const float pv = (t & 8) ? ((t & 1) ? p[0][3] : p[0][2]) : ((t & 1) ? p[0][1] : p[0][0]);
                         const float pt = __shfl_sync(0xffffffffu, pv, (lane & 28) + ((t & 7) >> 1));
                         if (pt != 0.0f)
 #pragma unroll
@@ -614,8 +683,8 @@ __global__ void __launch_bounds__(32 * kRowsWarps) attn_rows_kernel(const __grid
                 }
             }
             unsigned a[4];
-            split2(p[0], p[1], a[0], a[1]);
-            split2(p[2], p[3], a[2], a[3]);
+            split2(p[0][0], p[0][1], a[0], a[1]);
+            split2(p[0][2], p[0][3], a[2], a[3]);
 #pragma unroll
             for (int j = 0; j < NT / 2; ++j) {
                 unsigned b[4];
@@ -624,27 +693,43 @@ __global__ void __launch_bounds__(32 * kRowsWarps) attn_rows_kernel(const __grid
                 mma16816(o[2 * j + 1], a, b[2], b[3]);
             }
         } else {
-            unsigned w[4][(NB + 1) / 2];
+            const uint8_t* pp = vt + SL * T::kRow;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) lds_value_words<NB>(w[j], vt + (c + 4 * j) * T::kRow + g * 2 * NB);
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                float2 dm[4];
+            for (int u = 0; u < U; ++u) {
+                unsigned vp[4][NB], w[4][(NB + 1) / 2];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    dm[j] = __half22float2(*reinterpret_cast<__half2*>(&vp[j][b]));
-                    om[b] = fmaf(p[j], fmaf(8.0f, dm[j].x, dm[j].y), om[b]);
+                    lds_words(vp[j], pp + (u * 16 + slot_of<FMT>(c, j)) * T::kPar);
+                    lds_value_words<NB>(w[j], vt + (u * 16 + c + 4 * j) * T::kRow + g * 2 * NB);
                 }
-                unsigned a[4];
-                split2(p[0] * dm[0].x, p[1] * dm[1].x, a[0], a[1]);
-                split2(p[2] * dm[2].x, p[3] * dm[3].x, a[2], a[3]);
-                const unsigned sel = b & 1 ? 0x7632u : 0x5410u;
-                const unsigned x0 = __byte_perm(w[0][b / 2], w[1][b / 2], sel), x1 = __byte_perm(w[2][b / 2], w[3][b / 2], sel);
-                const unsigned h0 = x0 >> 8, h1 = x1 >> 8;
-                mma16816(o[4 * b], a, code_pair<false, true>(x0), code_pair<false, true>(x1));
-                mma16816(o[4 * b + 1], a, code_pair<true, true>(x0), code_pair<true, true>(x1));
-                mma16816(o[4 * b + 2], a, code_pair<false, true>(h0), code_pair<false, true>(h1));
-                mma16816(o[4 * b + 3], a, code_pair<true, true>(h0), code_pair<true, true>(h1));
+                if (hides) {  // a hidden slot's scales may be anything (slots behind the last are zeros)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int b = 0; b < NB; ++b)
+                            if (p[u][j] == 0.0f) vp[j][b] = 0u;
+                }
+                const float2 p01 = make_float2(p[u][0], p[u][1]), p23 = make_float2(p[u][2], p[u][3]);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    float2 dm[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) dm[j] = __half22float2(*reinterpret_cast<__half2*>(&vp[j][b]));
+                    const float2 d01 = make_float2(dm[0].x, dm[1].x), d23 = make_float2(dm[2].x, dm[3].x);
+                    om[b] = fma2(p01, fma2(both(8.0f), d01, make_float2(dm[0].y, dm[1].y)), om[b]);
+                    om[b] = fma2(p23, fma2(both(8.0f), d23, make_float2(dm[2].y, dm[3].y)), om[b]);
+                    const float2 e01 = mul2(p01, d01), e23 = mul2(p23, d23);
+                    unsigned a[4];
+                    split2(e01.x, e01.y, a[0], a[1]);
+                    split2(e23.x, e23.y, a[2], a[3]);
+                    const unsigned sel = b & 1 ? 0x7632u : 0x5410u;
+                    const unsigned x0 = __byte_perm(w[0][b / 2], w[1][b / 2], sel), x1 = __byte_perm(w[2][b / 2], w[3][b / 2], sel);
+                    const unsigned h0 = x0 >> 8, h1 = x1 >> 8;
+                    mma16816(o[4 * b], a, code_pair<false, true>(x0), code_pair<false, true>(x1));
+                    mma16816(o[4 * b + 1], a, code_pair<true, true>(x0), code_pair<true, true>(x1));
+                    mma16816(o[4 * b + 2], a, code_pair<false, true>(h0), code_pair<false, true>(h1));
+                    mma16816(o[4 * b + 3], a, code_pair<true, true>(h0), code_pair<true, true>(h1));
+                }
             }
         }
     }
@@ -661,7 +746,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps) attn_rows_kernel(const __grid
     } else {
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const float mm = quad_sum(om[b]);
+            const float mm = quad_sum(om[b].x + om[b].y);
             float r[8];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -1301,6 +1386,14 @@ int attn_launch_tile(const AttnP& P, bool general, cudaStream_t st) {
     }
     return launch_status();
 }
+template <int D, int FMT, int MODE>
+int attn_launch_rows(const AttnP& P, cudaStream_t st) {
+    constexpr int smem = RowsCfg<D, FMT>::kSmem;
+    static PerDeviceFlag raised;
+    if (!raise_dynamic_smem(attn_rows_kernel<D, FMT, MODE>, smem, raised)) return KCB_LAUNCH_FAILURE;
+    attn_rows_kernel<D, FMT, MODE><<<dim3(P.nsplit, P.kv_heads * P.row_tiles, P.n_seqs), 32 * kRowsWarps, smem, st>>>(P);
+    return launch_status();
+}
 template <int D, int FMT>
 int attn_launch_kernels(const AttnP& P, bool general, AttnKernel which, cudaStream_t st) {
     if (which == AttnKernel::tc) {
@@ -1314,18 +1407,12 @@ int attn_launch_kernels(const AttnP& P, bool general, AttnKernel which, cudaStre
     } else if (which == AttnKernel::tile) {
         if (const int e = attn_launch_tile<D, FMT>(P, general, st); e != KCB_SUCCESS) return e;
     } else {
-        constexpr int smem = RowsCfg<D, FMT>::kSmem;
-        static PerDeviceFlag raised[2];
-        const dim3 grid(P.nsplit, P.kv_heads * P.row_tiles, P.n_seqs);
-        if (general) {
-            if (!raise_dynamic_smem(attn_rows_kernel<D, FMT, true>, smem, raised[0])) return KCB_LAUNCH_FAILURE;
-            attn_rows_kernel<D, FMT, true><<<grid, 32 * kRowsWarps, smem, st>>>(P);
-        } else {
-            if (!raise_dynamic_smem(attn_rows_kernel<D, FMT, false>, smem, raised[1])) return KCB_LAUNCH_FAILURE;
-            attn_rows_kernel<D, FMT, false><<<grid, 32 * kRowsWarps, smem, st>>>(P);
-        }
+        int e;
+        if (P.positions || P.q_doc || P.mask) e = attn_launch_rows<D, FMT, 2>(P, st);
+        else if (P.cap_out != 0.0f || P.bias_step != 0.0f) e = attn_launch_rows<D, FMT, 1>(P, st);
+        else e = attn_launch_rows<D, FMT, 0>(P, st);
+        if (e != KCB_SUCCESS) return e;
     }
-    if (int e = launch_status(); e != KCB_SUCCESS) return e;
     const int joins = P.nsplit > 1 ? P.rows : 0, weights = P.scores ? (P.cap + kWeightSlots - 1) / kWeightSlots : 0;
     if (joins + weights) {
         const int e = launch_dependent(attn_merge_kernel<D>, dim3(joins + weights, P.kv_heads, P.n_seqs), 128, 0, st, P, joins);

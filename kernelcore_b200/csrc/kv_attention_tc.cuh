@@ -132,28 +132,11 @@ __device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile
 
 // One answer for the whole warp.
 __device__ __forceinline__ bool warp_failed(volatile int* fail) { return __any_sync(0xffffffffu, *fail != 0); }
-// Packed fp32 pairs (one instruction for two values, each rounded as the scalar operation).
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    unsigned long long r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)), "l"(reinterpret_cast<unsigned long long&>(c)));
-    return reinterpret_cast<float2&>(r);
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    unsigned long long r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
-    return reinterpret_cast<float2&>(r);
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    unsigned long long r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
-    return reinterpret_cast<float2&>(r);
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
 // Capped scores: y = tanh(y c), c positive; the cap itself is multiplied later.  A power series for |u| < 0.3 (to u^9: 5e-8) or
 // 0.55 (to u^15, see tanh_series), elsewhere 1 - 2 / (e^2|u| + 1): there the difference costs one bit.  A warp takes the shortest
