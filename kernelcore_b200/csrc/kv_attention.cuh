@@ -290,8 +290,14 @@ struct DocTiles {
     }
     __device__ __forceinline__ int next(int i) const {  // the wanted tile behind tile i, nt if there is none
         const int sh = shift();
-        for (++i; i < nt && !(bits[(i >> sh) / 32] >> ((i >> sh) % 32) & 1u); ++i) {}
-        return i;
+        ++i;
+        while (i < nt) {
+            const int b = i >> sh;
+            const uint32_t w = bits[b / 32] >> (b % 32);
+            if (w & 1u) break;
+            i = (b + (w ? __ffs(w) - 1 : 32 - b % 32)) << sh;
+        }
+        return min(i, nt);
     }
 };
 
@@ -794,12 +800,13 @@ __global__ void __launch_bounds__(32 * kRowsWarps, FMT == 16 && D == 128 ? 2 : 1
 // One CTA per row: its warps take the splits in turn, then the warps' sums are joined through shared memory.
 // After a rows launch that also wants weights, further CTAs (blockIdx.x from `joins` on) turn 512 slots' scores into weights each:
 // weights[t] += sum over the rows of 2^(score - M) / L, the rows in order, no atomics.
-constexpr int kWeightSlots = 512;
+constexpr int kWeightSlots = 512, kMergeWarps = 8;
 template <int D>
-__global__ void __launch_bounds__(128) attn_merge_kernel(const __grid_constant__ AttnP P, int joins) {
-    constexpr int W = 4, Q = (D / 4 + 31) / 32;
+__global__ void __launch_bounds__(32 * kMergeWarps) attn_merge_kernel(const __grid_constant__ AttnP P, int joins) {
+    constexpr int W = kMergeWarps, Q = (D / 4 + 31) / 32;
     __shared__ float4 acc[W][D / 4];
     __shared__ float2 ml[kRowsMax];
+    static_assert(W <= kRowsMax);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int row = blockIdx.x, kvh = blockIdx.y, s = blockIdx.z;
     grid_dependency_wait();
@@ -823,8 +830,8 @@ __global__ void __launch_bounds__(128) attn_merge_kernel(const __grid_constant__
         float* w = P.weights + sh * P.cap;
         const float* sc = P.scores + sh * P.rows * P.cap;
 #pragma unroll
-        for (int i = 0; i < kWeightSlots / 128; ++i) {
-            const int t = t0 + i * 128 + threadIdx.x;
+        for (int i = 0; i < kWeightSlots / (32 * W); ++i) {
+            const int t = t0 + i * (32 * W) + threadIdx.x;
             if (t >= n) continue;
             float sum = 0.0f;
             for (int r = 0; r < P.rows; ++r) {
@@ -865,11 +872,13 @@ __global__ void __launch_bounds__(128) attn_merge_kernel(const __grid_constant__
         if (q * 32 + lane < D / 4) acc[warp][q * 32 + lane] = a[q];
     if (lane == 0) ml[warp] = make_float2(M, L);
     __syncthreads();
-    L = ml[0].y + ml[1].y + ml[2].y + ml[3].y;
+    L = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) L += ml[w].y;
     const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;
     const int tok = row / P.group, head = kvh * P.group + row % P.group;
     float* out = P.out + static_cast<size_t>(s) * P.o_seq + static_cast<size_t>(tok) * P.o_token + static_cast<size_t>(head) * P.o_head;
-    for (int x = threadIdx.x; x < D / 4; x += 128) {
+    for (int x = threadIdx.x; x < D / 4; x += 32 * W) {
         float4 r = acc[0][x];
 #pragma unroll
         for (int w = 1; w < W; ++w) {
@@ -1415,7 +1424,7 @@ int attn_launch_kernels(const AttnP& P, bool general, AttnKernel which, cudaStre
     }
     const int joins = P.nsplit > 1 ? P.rows : 0, weights = P.scores ? (P.cap + kWeightSlots - 1) / kWeightSlots : 0;
     if (joins + weights) {
-        const int e = launch_dependent(attn_merge_kernel<D>, dim3(joins + weights, P.kv_heads, P.n_seqs), 128, 0, st, P, joins);
+        const int e = launch_dependent(attn_merge_kernel<D>, dim3(joins + weights, P.kv_heads, P.n_seqs), 32 * kMergeWarps, 0, st, P, joins);
         if (e != KCB_SUCCESS) return e;
     }
     if (P.final_ml) {

@@ -231,35 +231,6 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
     auto next = [&](int i) { return docs ? doc_tiles.next(i) : i + 1; };  // the tile behind tile i that is wanted
     auto swz = [&](int rows, int r, int ch) { return (ch >> 3) * (rows * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4); };
 
-    float ysc = 0.0f;
-    if (wg < 2) {  // the rows' queries: warpgroup 0 stores the hi halves, warpgroup 1 the lo halves
-        const int r = tid & 127, row = row0 + r;
-        const bool valid = row < P.rows;
-        const int token = (valid ? row : 0) / P.group, head = kvh * P.group + (valid ? row : 0) % P.group;
-        const float4* qp = reinterpret_cast<const float4*>(P.q + static_cast<size_t>(s) * P.q_seq + static_cast<size_t>(token) * P.q_token + static_cast<size_t>(head) * P.q_head);
-        const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float amax = 0.0f;
-#pragma unroll 8
-        for (int i = 0; i < D / 4; ++i) {
-            const float4 f = valid ? qp[i] : zero;
-            amax = fmaxf(fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y))), fmaxf(fabsf(f.z), fabsf(f.w)));
-        }
-        float up, down;
-        row_scale(amax, up, down);
-        ysc = fmaxf(fabsf(P.sc) * down, 1e-37f);  // positive, so that the largest product is the largest score; a negative scale goes to the query
-        if (P.sc < 0.0f) up = -up;
-#pragma unroll 4
-        for (int ch = 0; ch < CH; ++ch) {
-            const float4 a = valid ? qp[2 * ch] : zero, b = valid ? qp[2 * ch + 1] : zero;
-            uint4 hi, lo;
-            split2(a.x * up, a.y * up, hi.x, lo.x);
-            split2(a.z * up, a.w * up, hi.y, lo.y);
-            split2(b.x * up, b.y * up, hi.z, lo.z);
-            split2(b.z * up, b.w * up, hi.w, lo.w);
-            *reinterpret_cast<uint4*>(sm + wg * C::kQHalf + swz(C::kRows, r, ch)) = wg ? lo : hi;
-        }
-        fence_async_shared();
-    }
     tc_before_sync();
     __syncthreads();
     tc_after_sync();
@@ -282,6 +253,7 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
                     auto scores = [&](int j) {  // (hi + lo) keys^T, both halves of the tile
                         const int st = j % C::kStages;
                         tc_wait(&kfull[st], (j / C::kStages) & 1, fail);
+                        if (j == 0) named_sync(5, 288);  // the queries are there
                         __syncwarp();
                         tc_after_sync();
                         if (warp_failed(fail)) return;
@@ -299,6 +271,7 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
                     };
                     int tile = next(-1);
                     if (tile < nt) scores(i);
+                    else if (!careful) named_sync(5, 288);
                     while (tile < nt) {
                         tile = next(tile);
                         tc_wait(sread, i & 1, fail);
@@ -458,6 +431,32 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsSoftmax));
         const int r = tid & 127, row = row0 + r;
         const bool valid = row < P.rows;
+        // the rows' queries: warpgroup 0 stores the hi halves, warpgroup 1 the lo halves
+        const int token = (valid ? row : 0) / P.group, head = kvh * P.group + (valid ? row : 0) % P.group;
+        const float4* qp = reinterpret_cast<const float4*>(P.q + static_cast<size_t>(s) * P.q_seq + static_cast<size_t>(token) * P.q_token + static_cast<size_t>(head) * P.q_head);
+        const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float amax = 0.0f;
+#pragma unroll 8
+        for (int i = 0; i < D / 4; ++i) {
+            const float4 f = valid ? qp[i] : zero;
+            amax = fmaxf(fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y))), fmaxf(fabsf(f.z), fabsf(f.w)));
+        }
+        float up, down;
+        row_scale(amax, up, down);
+        const float ysc = fmaxf(fabsf(P.sc) * down, 1e-37f);  // positive, so that the largest product is the largest score; a negative scale goes to the query
+        if (P.sc < 0.0f) up = -up;
+#pragma unroll 4
+        for (int ch = 0; ch < CH; ++ch) {
+            const float4 a = valid ? qp[2 * ch] : zero, b = valid ? qp[2 * ch + 1] : zero;
+            uint4 hi, lo;
+            split2(a.x * up, a.y * up, hi.x, lo.x);
+            split2(a.z * up, a.w * up, hi.y, lo.y);
+            split2(b.x * up, b.y * up, hi.z, lo.z);
+            split2(b.z * up, b.w * up, hi.w, lo.w);
+            *reinterpret_cast<uint4*>(sm + wg * C::kQHalf + swz(C::kRows, r, ch)) = wg ? lo : hi;
+        }
+        fence_async_shared();
+        named_sync(5, 288);
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + C::kS + wg * HK + lanes, to = tmem + C::kO + wg * (D / 2) + lanes;
         float* maxima = reinterpret_cast<float*>(sm + C::kMax);

@@ -21,13 +21,34 @@ namespace {
 // Bounded by memory: 4 bytes read and 2 or 0.625 written per value.  Eight lanes hold a block of 32 channels, so a warp reads
 // 512 contiguous bytes and reduces minima and maxima in three shuffle steps.
 // The code is rounded from the exact quotient: the fp32 quotient decides unless it lies near a half, where fp64 does.
-__device__ __forceinline__ unsigned code_of(float x, float m, float d, float inv) {
-    const float t = (x - m) * inv;
-    float r = rintf(t);
-    // t is off by at most 16 * 3 * 2^-24 < 3e-6; between 0.4999 and 0.5001 from an integer the quotient is taken in 64 bits
-    if (fabsf(fabsf(t - r) - 0.5f) < 1e-4f) r = static_cast<float>(rint((static_cast<double>(x) - static_cast<double>(m)) / static_cast<double>(d)));
-    return static_cast<unsigned>(static_cast<int>(fminf(fmaxf(r, 0.0f), 15.0f)));
+__device__ __forceinline__ unsigned codes_of(const float (&x)[4], float m, float d, float inv) {
+    constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to the nearest integer, to even at ties, into the low bits
+    unsigned w = 0;
+    float far = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float t = fminf(fmaxf((x[k] - m) * inv, 0.0f), 15.0f), z = t + kMagic;
+        far = fmaxf(far, fabsf(t - (z - kMagic)));
+        w |= (__float_as_uint(z) & 15u) << (4 * k);
+    }
+    // t is off by at most 16 * 3 * 2^-24 < 3e-6: nearer than 1e-4 to a half the quotient is taken in 64 bits
+    if (far > 0.4999f) {
+        w = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const double r = rint((static_cast<double>(x[k]) - static_cast<double>(m)) / static_cast<double>(d));
+            w |= static_cast<unsigned>(fmin(fmax(r, 0.0), 15.0)) << (4 * k);
+        }
+    }
+    return w;
 }
+// x / d by a multiplication: `inv` = ceil(2^32 / d) gives the quotient or one more for every x below 2^31.
+__device__ __forceinline__ unsigned divide(unsigned x, unsigned d, unsigned inv) {
+    if (d == 1) return x;
+    const unsigned q = __umulhi(x, inv);
+    return q * d > x ? q - 1 : q;
+}
+inline unsigned divisor(unsigned d) { return static_cast<unsigned>((0x100000000ull + d - 1) / d); }
 // Where a row's four channels 4 jr .. 4 jr + 3 stand in the 4-bit planes: the two bytes of codes, the block's parameters.
 struct Q4Place {
     size_t codes, params;
@@ -43,6 +64,7 @@ struct AppendP {
     const float* k;
     const float* v;
     long long tok, seq, seq_bytes, par_off;
+    unsigned heads_inv;
     int n_tokens, count;  // count: this launch also moves the counts on (one CTA per sequence)
 };
 __device__ __forceinline__ float cache_value(float x) {  // what a cache can hold: NaN -> 0, the rest within fp16's range
@@ -70,7 +92,7 @@ __global__ void __launch_bounds__(kRowThreads) kv_append_rows_kernel(const __gri
 #pragma unroll
         for (int i = 0; i < kRowIter; ++i) {
             const unsigned r = base + i * per_cta + r0, x = r < rows ? r : r - rows;
-            tt[i] = x / c.kv_heads, hh[i] = x % c.kv_heads;
+            tt[i] = divide(x, c.kv_heads, A.heads_inv), hh[i] = x - tt[i] * c.kv_heads;
             f[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (live && r < 2 * rows) f[i] = *reinterpret_cast<const float4*>((r < rows ? A.k : A.v) + s * A.seq + tt[i] * A.tok + static_cast<long long>(hh[i]) * c.head_dim + 4 * jr);
         }
@@ -93,10 +115,7 @@ __global__ void __launch_bounds__(kRowThreads) kv_append_rows_kernel(const __gri
                 for (int o = 1; o < 8; o <<= 1) lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o)), hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
                 const __half mh = __float2half_rn(lo), dh = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
                 const float m = __half2float(mh), d = __half2float(dh), inv = d > 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
-                unsigned w = 0;
-                if (d > 0.0f)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) w |= code_of(e[k], m, d, inv) << (4 * k);
+                const unsigned w = d > 0.0f ? codes_of(e, m, d, inv) : 0u;
                 if (put) {
                     uint8_t* plane = static_cast<uint8_t*>(val ? c.v : c.k) + A.seq_bytes * s;
                     const Q4Place at = q4_place(c, A.par_off, val, h, t, jr);
@@ -128,6 +147,7 @@ struct ReadP {
     float* k;
     float* v;
     long long seq_bytes, par_off;
+    unsigned heads_inv;
     int first, count;
 };
 template <int BITS>
@@ -144,8 +164,9 @@ __global__ void __launch_bounds__(kRowThreads) kv_read_rows_kernel(const __grid_
         for (int i = 0; i < kRowIter; ++i) {
             const unsigned r = base + i * per_cta + r0, x = r < rows ? r : r - rows;
             const bool val = r >= rows;
-            const long long t = static_cast<long long>(R.first) + x / c.kv_heads;
-            const int h = static_cast<int>(x % c.kv_heads);
+            const unsigned tok = divide(x, c.kv_heads, R.heads_inv);
+            const long long t = static_cast<long long>(R.first) + tok;
+            const int h = static_cast<int>(x - tok * c.kv_heads);
             w[i] = make_uint2(0u, 0u);
             if (r >= 2 * rows || t >= n) continue;
             if (BITS == 16) {
@@ -219,7 +240,7 @@ __device__ __forceinline__ int warp_prefix(int v, int* slots, int& total) {
 }
 __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_constant__ EvictP E) {
     extern __shared__ unsigned keys[];
-    __shared__ int hist[4][256], slots[33], digit, rest;
+    __shared__ int hist[2048], slots[33], digit, rest;
     const kcb_kv_cache& c = E.c;
     const int h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const size_t sh = static_cast<size_t>(s) * c.kv_heads + h;
@@ -235,50 +256,44 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_con
     const bool held = n <= kSelKeys;
     auto make_key = [&](int t) { return pos[t] >= from ? 0xFFFFFFFFu : weight_key(w[t]); };
     auto key_of = [&](int t) { return held ? keys[t] : make_key(t); };
-    (&hist[0][0])[tid] = 0;
-    __syncthreads();
-#pragma unroll 4
-    for (int t = tid; t < n; t += kSelThreads) {
-        const unsigned k = make_key(t);
-        if (held) keys[t] = k;
-        atomicAdd(&hist[3][k >> 24], 1);
-    }
-    __syncthreads();
+    // three digits of 11, 11 and 10 bits, from the top: so wide that the weights of a cache, which share few exponents, spread over
+    // many counters
     unsigned prefix = 0, mask = 0;
     int need = keep;
-    for (int round = 3; round >= 0; --round) {
-        const int shift = 8 * round;
-        if (round < 3) {
+#pragma unroll 1
+    for (int round = 0; round < 3; ++round) {
+        const int shift = round == 0 ? 21 : round == 1 ? 10 : 0, bins = round < 2 ? 2048 : 1024;
+        hist[tid] = 0, hist[tid + 1024] = 0;
+        __syncthreads();
 #pragma unroll 4
-            for (int t = tid; t < n; t += kSelThreads) {
-                const unsigned k = key_of(t);
-                if ((k & mask) == prefix) atomicAdd(&hist[round][k >> shift & 255u], 1);
+        for (int t = tid; t < n; t += kSelThreads) {
+            unsigned k;
+            if (round == 0) {
+                k = make_key(t);
+                if (held) keys[t] = k;
+            } else {
+                k = key_of(t);
             }
-            __syncthreads();
+            if ((k & mask) == prefix) atomicAdd(&hist[k >> shift & (bins - 1)], 1);
         }
-        if (tid < 32) {  // from the largest digit down: where does the need-th key fall?
-            int mine[8], sum = 0;
+        __syncthreads();
+        // from the largest digit down, two to a thread: where does the need-th key fall?
+        const int a = bins - 1 - 2 * tid, ha = a > 0 ? hist[a] : 0, hb = a > 0 ? hist[a - 1] : 0;
+        int before = ha + hb;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum += mine[i] = hist[round][255 - (tid * 8 + i)];
-            int before = sum;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, before, o);
-                if (tid >= o) before += y;
-            }
-            before -= sum;
-            if (before < need && need <= before + sum) {
-                int left = need - before;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (left > 0 && left <= mine[i]) digit = 255 - (tid * 8 + i), rest = left;
-                    left -= mine[i];
-                }
-            }
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += y;
+        }
+        int all;
+        before += warp_prefix(__shfl_sync(0xffffffffu, before, 31), slots, all) - (ha + hb);
+        if (before < need && need <= before + ha + hb) {
+            const bool first = need - before <= ha;
+            digit = first ? a : a - 1, rest = need - before - (first ? 0 : ha);
         }
         __syncthreads();
         prefix |= static_cast<unsigned>(digit) << shift;
-        mask |= 255u << shift;
+        mask |= static_cast<unsigned>(bins - 1) << shift;
         need = rest;
         __syncthreads();
     }
@@ -415,7 +430,7 @@ AttnCut attn_cut(const kcb_kv_cache* c, const kcb_cache_attn* a) {
     const int per = r.which == AttnKernel::rows ? 8 : r.which == AttnKernel::tile ? 64 : 128;
     r.row_tiles = static_cast<int>((rows + per - 1) / per);
     const long long ctas = static_cast<long long>(c->n_seqs) * c->kv_heads * r.row_tiles;
-    const long long want = (r.which == AttnKernel::rows ? 4 : r.which == AttnKernel::tile ? 2 : 1) * kSmCount, least = r.which == AttnKernel::rows ? 256 : 512;
+    const long long want = (r.which == AttnKernel::rows ? (c->n_seqs == 1 ? 2 : 4) : r.which == AttnKernel::tile ? 2 : 1) * kSmCount, least = r.which == AttnKernel::rows ? 128 : 512;
     r.nsplit = static_cast<int>(std::max<long long>(1, std::min<long long>(want / std::max<long long>(ctas, 1), (c->capacity + least - 1) / least)));
     // partial sums where keys are split; for weights the rows' final sums (tiles) or every score and the partial sums (rows)
     const size_t all = static_cast<size_t>(c->n_seqs) * c->kv_heads * rows;
@@ -472,7 +487,7 @@ int kcb_cache_append(const kcb_kv_cache* c, const float* k, const float* v, int 
     const unsigned blocks = row_blocks(c, n_tokens);
     const bool one = blocks <= 4;  // a step's few rows: one CTA per sequence, which also moves the counts on
     AppendP A{*c, k, v, token_stride, seq_stride, static_cast<long long>(q4_seq_bytes(c->kv_heads, c->head_dim, c->capacity)),
-              static_cast<long long>(q4_param_offset(c->kv_heads, c->head_dim, c->capacity)), n_tokens, one};
+              static_cast<long long>(q4_param_offset(c->kv_heads, c->head_dim, c->capacity)), divisor(c->kv_heads), n_tokens, one};
     const dim3 grid(one ? 1 : blocks, c->n_seqs);
     if (c->bits == KCB_CACHE_F16) kv_append_rows_kernel<16><<<grid, kRowThreads, 0, st>>>(A);
     else kv_append_rows_kernel<4><<<grid, kRowThreads, 0, st>>>(A);
@@ -488,7 +503,7 @@ int kcb_cache_read(const kcb_kv_cache* c, int first, int count, float* k_out, fl
     if (count == 0 || c->n_seqs == 0) return KCB_SUCCESS;
     const auto st = static_cast<cudaStream_t>(stream);
     ReadP R{*c, k_out, v_out, static_cast<long long>(q4_seq_bytes(c->kv_heads, c->head_dim, c->capacity)),
-            static_cast<long long>(q4_param_offset(c->kv_heads, c->head_dim, c->capacity)), first, count};
+            static_cast<long long>(q4_param_offset(c->kv_heads, c->head_dim, c->capacity)), divisor(c->kv_heads), first, count};
     const dim3 grid(row_blocks(c, count), c->n_seqs);
     if (c->bits == KCB_CACHE_F16) kv_read_rows_kernel<16><<<grid, kRowThreads, 0, st>>>(R);
     else kv_read_rows_kernel<4><<<grid, kRowThreads, 0, st>>>(R);
