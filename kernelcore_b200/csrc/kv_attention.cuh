@@ -798,9 +798,9 @@ __global__ void __launch_bounds__(32 * kRowsWarps, FMT == 16 && D == 128 ? 2 : 1
 
 // ---- joining the splits of a row -------------------------------------------------------------------------------------------
 // One CTA per row: its warps take the splits in turn, then the warps' sums are joined through shared memory.
-// After a rows launch that also wants weights, further CTAs (blockIdx.x from `joins` on) turn 512 slots' scores into weights each:
+// After a rows launch that also wants weights, further CTAs (blockIdx.x from `joins` on) turn 2048 slots' scores into weights each:
 // weights[t] += sum over the rows of 2^(score - M) / L, the rows in order, no atomics.
-constexpr int kWeightSlots = 512, kMergeWarps = 8;
+constexpr int kWeightSlots = 2048, kMergeWarps = 8;
 template <int D>
 __global__ void __launch_bounds__(32 * kMergeWarps) attn_merge_kernel(const __grid_constant__ AttnP P, int joins) {
     constexpr int W = kMergeWarps, Q = (D / 4 + 31) / 32;
@@ -829,16 +829,25 @@ __global__ void __launch_bounds__(32 * kMergeWarps) attn_merge_kernel(const __gr
         __syncthreads();
         float* w = P.weights + sh * P.cap;
         const float* sc = P.scores + sh * P.rows * P.cap;
+        constexpr int kPer = kWeightSlots / (32 * W);  // slots per thread, all of a row's scores requested at once
+        float sum[kPer];
 #pragma unroll
-        for (int i = 0; i < kWeightSlots / (32 * W); ++i) {
-            const int t = t0 + i * (32 * W) + threadIdx.x;
-            if (t >= n) continue;
-            float sum = 0.0f;
-            for (int r = 0; r < P.rows; ++r) {
-                const float y = sc[static_cast<size_t>(r) * P.cap + t];
-                if (y != -INFINITY) sum = fmaf(ex2(y - ml[r].x), ml[r].y, sum);
+        for (int i = 0; i < kPer; ++i) sum[i] = 0.0f;
+        for (int r = 0; r < P.rows; ++r) {
+            float y[kPer];
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int t = t0 + i * (32 * W) + threadIdx.x;
+                y[i] = t < n ? sc[static_cast<size_t>(r) * P.cap + t] : -INFINITY;
             }
-            w[t] += sum;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+                if (y[i] != -INFINITY) sum[i] = fmaf(ex2(y[i] - ml[r].x), ml[r].y, sum[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int t = t0 + i * (32 * W) + threadIdx.x;
+            if (t < n) w[t] += sum[i];
         }
         return;
     }

@@ -431,35 +431,53 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsSoftmax));
         const int r = tid & 127, row = row0 + r;
         const bool valid = row < P.rows;
-        // the rows' queries: warpgroup 0 stores the hi halves, warpgroup 1 the lo halves
-        const int token = (valid ? row : 0) / P.group, head = kvh * P.group + (valid ? row : 0) % P.group;
-        const float4* qp = reinterpret_cast<const float4*>(P.q + static_cast<size_t>(s) * P.q_seq + static_cast<size_t>(token) * P.q_token + static_cast<size_t>(head) * P.q_head);
-        const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float amax = 0.0f;
-#pragma unroll 8
-        for (int i = 0; i < D / 4; ++i) {
-            const float4 f = valid ? qp[i] : zero;
-            amax = fmaxf(fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y))), fmaxf(fabsf(f.z), fabsf(f.w)));
+        float* maxima = reinterpret_cast<float*>(sm + C::kMax);
+        {  // the queries as hi and lo tiles, and each row's factor: eight lanes to a row, so that rows are read in whole lines
+            const int l8 = tid & 7;
+#pragma unroll 1
+            for (int q = tid >> 3; q < C::kRows; q += 32) {
+                const int qrow = row0 + q;
+                const bool ok = qrow < P.rows;
+                const int token = (ok ? qrow : 0) / P.group, head = kvh * P.group + (ok ? qrow : 0) % P.group;
+                const float4* qp = reinterpret_cast<const float4*>(P.q + static_cast<size_t>(s) * P.q_seq + static_cast<size_t>(token) * P.q_token + static_cast<size_t>(head) * P.q_head);
+                constexpr int kPer = CH / 8;  // pieces of 8 channels per lane
+                float4 x[kPer][2];
+                float amax = 0.0f;
+#pragma unroll
+                for (int k = 0; k < kPer; ++k)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float4 f = ok ? qp[2 * (k * 8 + l8) + e] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        x[k][e] = f;
+                        amax = fmaxf(fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y))), fmaxf(fabsf(f.z), fabsf(f.w)));
+                    }
+#pragma unroll
+                for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                float up, down;
+                row_scale(amax, up, down);
+                // positive, so that the largest product is the largest score; a negative scale goes to the query
+                if (l8 == 0) maxima[q] = fmaxf(fabsf(P.sc) * down, 1e-37f);
+                if (P.sc < 0.0f) up = -up;
+#pragma unroll
+                for (int k = 0; k < kPer; ++k) {
+                    const float4 a = x[k][0], b = x[k][1];
+                    uint4 hi, lo;
+                    split2(a.x * up, a.y * up, hi.x, lo.x);
+                    split2(a.z * up, a.w * up, hi.y, lo.y);
+                    split2(b.x * up, b.y * up, hi.z, lo.z);
+                    split2(b.z * up, b.w * up, hi.w, lo.w);
+                    const int at = swz(C::kRows, q, k * 8 + l8);
+                    *reinterpret_cast<uint4*>(sm + at) = hi;
+                    *reinterpret_cast<uint4*>(sm + C::kQHalf + at) = lo;
+                }
+            }
+            fence_async_shared();
         }
-        float up, down;
-        row_scale(amax, up, down);
-        const float ysc = fmaxf(fabsf(P.sc) * down, 1e-37f);  // positive, so that the largest product is the largest score; a negative scale goes to the query
-        if (P.sc < 0.0f) up = -up;
-#pragma unroll 4
-        for (int ch = 0; ch < CH; ++ch) {
-            const float4 a = valid ? qp[2 * ch] : zero, b = valid ? qp[2 * ch + 1] : zero;
-            uint4 hi, lo;
-            split2(a.x * up, a.y * up, hi.x, lo.x);
-            split2(a.z * up, a.w * up, hi.y, lo.y);
-            split2(b.x * up, b.y * up, hi.z, lo.z);
-            split2(b.z * up, b.w * up, hi.w, lo.w);
-            *reinterpret_cast<uint4*>(sm + wg * C::kQHalf + swz(C::kRows, r, ch)) = wg ? lo : hi;
-        }
-        fence_async_shared();
         named_sync(5, 288);
+        const float ysc = maxima[r];
+        named_sync(4, 256);  // the maxima of the first tile go to the same place
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + C::kS + wg * HK + lanes, to = tmem + C::kO + wg * (D / 2) + lanes;
-        float* maxima = reinterpret_cast<float*>(sm + C::kMax);
         RowInfo ri{};
         if (GEN) ri = row_info(P, s, kvh, n, row);
         // slots from `limit` on are hidden by the end of the range, or (slot = position) by causality
@@ -672,23 +690,27 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
         maxima[wg * C::kRows + r] = l;
         named_sync(4, 256);
         const float L = l + maxima[(1 - wg) * C::kRows + r];
-        const size_t part = ((static_cast<size_t>(s) * P.kv_heads + kvh) * P.nsplit + split) * P.rows + row;
-        if (valid) {
-            float* dst;
-            float f = 1.0f;
-            if (P.nsplit > 1) {
-                dst = P.part_o + part * D;
-            } else {
-                f = L > 0.0f || L != L ? 1.0f / L : 0.0f;
-                const int token = row / P.group, head = kvh * P.group + row % P.group;
-                dst = P.out + static_cast<size_t>(s) * P.o_seq + static_cast<size_t>(token) * P.o_token + static_cast<size_t>(head) * P.o_head;
-            }
+        const float f = P.nsplit > 1 ? 1.0f : L > 0.0f || L != L ? 1.0f / L : 0.0f;
+        // through shared memory (the rings are free), so that rows are written in whole lines
+        constexpr int kStride = D + 4;
+        static_assert(C::kRows * kStride * 4 <= 2 * C::kStages * C::kSlot, "the rings hold the output");
+        float* stage_out = reinterpret_cast<float*>(sm + C::kOffK);
 #pragma unroll
-            for (int k = 0; k < D / 4; k += 2) *reinterpret_cast<float4*>(dst + wg * (D / 2) + 2 * k) = make_float4(o[k].x * f, o[k].y * f, o[k + 1].x * f, o[k + 1].y * f);
-            if (wg == 0) {
-                if (P.nsplit > 1) P.part_ml[part] = make_float2(m, L);
-                else if (P.final_ml) P.final_ml[(static_cast<size_t>(s) * P.kv_heads + kvh) * P.rows + row] = make_float2(m, L);
-            }
+        for (int k = 0; k < D / 4; k += 2)
+            *reinterpret_cast<float4*>(stage_out + r * kStride + wg * (D / 2) + 2 * k) = make_float4(o[k].x * f, o[k].y * f, o[k + 1].x * f, o[k + 1].y * f);
+        const size_t part0 = ((static_cast<size_t>(s) * P.kv_heads + kvh) * P.nsplit + split) * P.rows;
+        if (wg == 0 && valid) {
+            if (P.nsplit > 1) P.part_ml[part0 + row] = make_float2(m, L);
+            else if (P.final_ml) P.final_ml[(static_cast<size_t>(s) * P.kv_heads + kvh) * P.rows + row] = make_float2(m, L);
+        }
+        named_sync(4, 256);
+        for (int x = tid; x < C::kRows * (D / 4); x += 256) {
+            const int q = x / (D / 4), ch = x % (D / 4) * 4, qrow = row0 + q;
+            if (qrow >= P.rows) break;
+            const int token = qrow / P.group, head = kvh * P.group + qrow % P.group;
+            float* dst = P.nsplit > 1 ? P.part_o + (part0 + qrow) * D
+                                      : P.out + static_cast<size_t>(s) * P.o_seq + static_cast<size_t>(token) * P.o_token + static_cast<size_t>(head) * P.o_head;
+            *reinterpret_cast<float4*>(dst + ch) = *reinterpret_cast<const float4*>(stage_out + q * kStride + ch);
         }
     }
     // ---- teardown: nothing of this CTA is in flight when its TMEM goes back ---------------------------------------------------
