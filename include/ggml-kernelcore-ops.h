@@ -64,6 +64,8 @@ int kcb_ggml_swiglu(void* ctx, const kcb_tensor* dst);                  /* swigl
 int kcb_ggml_fused_swiglu(void* ctx, const kcb_tensor* dst);            /* fused_swiglu   :525-534 */
 int kcb_ggml_set_rows(void* ctx, const kcb_tensor* dst);                /* set_rows       :664-674 */
 int kcb_ggml_flash_attn(void* ctx, const kcb_tensor* dst);              /* flash_attn     :677-711 */
+/* (op_params 1 and 2, max_bias and logit_softcap, which the reference's backend does not take, go to kcb_cache_attention;
+ * its alignment and head dimensions hold then.) */
 
 #ifdef __cplusplus
 }

@@ -288,7 +288,7 @@ int kcb_flash_attn_f16(const float* q_dev, const void* k_dev, const void* v_dev,
  *            [kv_heads][capacity][head_dim / 2], then {d, m} as fp16 [kv_heads][capacity][head_dim / 32][2].  A key row
  *            holds for c = 0..3 the 4 bytes of channels 8c..8c+7 of every block, a value row for g = 0..7 the 2 bytes
  *            of channels 4g..4g+3 of every block; two channels to a byte, the lower one in the low nibble.
- * n_keys[seq]: rows in use (slots 0 .. n_keys - 1; what lies behind is never read); NULL: all `capacity` rows.
+ * n_keys[seq]: rows in use (slots 0 .. n_keys - 1; what lies behind has no effect, whatever it is); NULL: all `capacity` rows.
  * next_pos[seq]: tokens seen so far, the position of the next one; NULL: n_keys (nothing was evicted).
  * positions[seq][head][slot]: the position of the row in a slot; NULL: slot = position.
  * weights[seq][head][slot]: attention weight the row has received so far. */

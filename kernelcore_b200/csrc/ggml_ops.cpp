@@ -300,6 +300,24 @@ int kcb_ggml_flash_attn(void* h, const kcb_tensor* dst) {
     const int D = static_cast<int>(k->ne[0]), T = static_cast<int>(k->ne[1]), Hkv = static_cast<int>(k->ne[2]);
     const int H = static_cast<int>(q->ne[2]), N = static_cast<int>(q->ne[1]);
     if (Hkv <= 0 || H % Hkv) return KCB_INVALID_VALUE;
+    const float max_bias = param_f32(dst, 1), softcap = param_f32(dst, 2);
+    if (max_bias != 0.0f || softcap != 0.0f) {  // capped or distance-biased scores: the KV-cache attention
+        auto& c = *static_cast<Ctx*>(h);
+        kcb_kv_cache cache{};
+        cache.bits = KCB_CACHE_F16, cache.n_seqs = 1, cache.kv_heads = Hkv, cache.head_dim = D, cache.capacity = T;
+        cache.k = k->data, cache.v = v->data;
+        cache.k_row = static_cast<int64_t>(k->nb[1] / 2), cache.k_head = static_cast<int64_t>(k->nb[2] / 2);
+        cache.v_row = static_cast<int64_t>(v->nb[1] / 2), cache.v_head = static_cast<int64_t>(v->nb[2] / 2);
+        kcb_cache_attn a{};
+        a.n_tokens = N, a.heads = H, a.scale = param_f32(dst, 0), a.softcap = softcap, a.max_bias = max_bias;
+        a.mask = mask ? mask->data : nullptr, a.mask_token = mask ? static_cast<int64_t>(mask->nb[1] / 2) : 0;
+        a.q_token = static_cast<int64_t>(q->nb[1] / 4), a.q_head = static_cast<int64_t>(q->nb[2] / 4);
+        a.out_token = static_cast<int64_t>(H) * D, a.out_head = D;
+        const size_t ws = kcb_cache_attention_workspace_bytes(&cache, &a);
+        int* scratch = ws ? c.take((ws + 3) / 4) : nullptr;
+        if (ws && !scratch) return KCB_OUT_OF_MEMORY;
+        return kcb_cache_attention(&cache, &a, f32(q), f32w(dst), scratch, ws, c.stream);
+    }
     // field order of llm::FaDims (llm/llm_kernels.hpp:316-332); K, V and mask strides in 32-bit words, q strides in floats
     d[0] = H, d[1] = T, d[2] = D, d[3] = H / Hkv, d[4] = (T + 7) / 8 * 8;
     d[5] = static_cast<int>(k->nb[1] / 4), d[6] = static_cast<int>(k->nb[2] / 4);

@@ -208,6 +208,8 @@ __device__ __forceinline__ int row_pos(const AttnP& P, int s, int n, int token) 
     if (P.q_pos) return P.q_pos[static_cast<size_t>(s) * P.n_tokens + token];
     return (P.next_pos ? P.next_pos[s] : n) - P.n_tokens + token;
 }
+// Slots (= positions) from here on are hidden from a row by causality; `end` bounds it.
+__device__ __forceinline__ int causal_limit(int pos, int prefix, int end) { return pos >= end ? end : min(end, max(prefix, pos + 1)); }
 __device__ __forceinline__ RowInfo row_info(const AttnP& P, int s, int kvh, int n, int row) {
     RowInfo r;
     r.valid = row < P.rows;
@@ -243,7 +245,7 @@ __device__ __forceinline__ float general_score(const AttnP& P, float z, const Ro
         see = see && add != -INFINITY;  // hides whatever the product is
         y += r.slope * add;
     } else if (P.bias_step != 0.0f) {
-        y -= r.slope * fabsf(static_cast<float>(r.pos) - static_cast<float>(key.pos));
+        y -= r.slope * fabsf(static_cast<float>(r.pos - key.pos));
     }
     return see ? y : -INFINITY;
 }
@@ -541,9 +543,8 @@ __global__ void __launch_bounds__(32 * kRowsWarps, FMT == 16 && D == 128 ? 2 : 1
     int limit = valid ? end : 0;
     const int prefix = P.prefix ? P.prefix[s] : 0;
     if (MODE) ri = row_info(P, s, kvh, n, row);
-    if (MODE < 2 && P.causal && valid) limit = min(end, max(prefix, row_pos(P, s, n, token) + 1));
+    if (MODE < 2 && P.causal && valid) limit = causal_limit(row_pos(P, s, n, token), prefix, end);
     const bool hides = MODE == 2 || (P.causal && (P.n_tokens > 1 || P.next_pos || P.q_pos));  // slots in use may be hidden from a row
-    const float rpos = static_cast<float>(ri.pos);
 
     float o[NT][4], m = -INFINITY, l = 0.0f;
     float2 om[FMT == 16 ? 1 : NB];
@@ -611,7 +612,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps, FMT == 16 && D == 128 ? 2 : 1
                 } else {
                     if (MODE == 1) {
                         if (P.cap_out != 0.0f) v = tanh_acc(v) * P.cap_out;
-                        if (P.bias_step != 0.0f) v -= ri.slope * fabsf(rpos - static_cast<float>(t));
+                        if (P.bias_step != 0.0f) v -= ri.slope * fabsf(static_cast<float>(ri.pos - t));
                     }
                     if (t >= limit) v = -INFINITY;
                 }
@@ -1063,7 +1064,7 @@ __global__ void __launch_bounds__(128) attn_tile_kernel(const __grid_constant__ 
     const int tok0 = row0 / P.group, tok1 = last_row / P.group;
     const int prefix = GEN && P.prefix ? P.prefix[s] : 0;
     if (P.causal && !P.positions && !P.q_pos)  // no row here sees a slot behind the last token's position or the prefix
-        end = max(begin, min(end, max(prefix, row_pos(P, s, n, tok1) + 1)));
+        end = max(begin, causal_limit(row_pos(P, s, n, tok1), prefix, end));
     const int nt = (end - begin + TK - 1) / TK;
 
     const bool docs = GEN && P.q_doc != nullptr;
@@ -1091,8 +1092,8 @@ __global__ void __launch_bounds__(128) attn_tile_kernel(const __grid_constant__ 
         ia = row_info(P, s, kvh, n, ra), ib = row_info(P, s, kvh, n, rb);
     } else {
         if (P.causal) {
-            lima = ra < P.rows ? min(n, row_pos(P, s, n, ra / P.group) + 1) : 0;
-            limb = rb < P.rows ? min(n, row_pos(P, s, n, rb / P.group) + 1) : 0;
+            lima = ra < P.rows ? causal_limit(row_pos(P, s, n, ra / P.group), 0, n) : 0;
+            limb = rb < P.rows ? causal_limit(row_pos(P, s, n, rb / P.group), 0, n) : 0;
         }
     }
     const float* yscp = reinterpret_cast<const float*>(sm + Q::kYsc) + warp * 16 + g;

@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
     int end = min(n, begin + chunk);
     const int tok0 = row0 / P.group, tok1 = (min(P.rows, row0 + C::kRows) - 1) / P.group;
     const int prefix = P.prefix ? P.prefix[s] : 0;
-    if (P.causal && !P.positions && !P.q_pos) end = max(begin, min(end, max(prefix, row_pos(P, s, n, tok1) + 1)));
+    if (P.causal && !P.positions && !P.q_pos) end = max(begin, causal_limit(row_pos(P, s, n, tok1), prefix, end));
     const int nt = (end - begin + KT - 1) / KT;
     const bool docs = GEN && P.q_doc != nullptr;
 
@@ -434,23 +434,28 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
         float* maxima = reinterpret_cast<float*>(sm + C::kMax);
         {  // the queries as hi and lo tiles, and each row's factor: eight lanes to a row, so that rows are read in whole lines
             const int l8 = tid & 7;
-#pragma unroll 1
-            for (int q = tid >> 3; q < C::kRows; q += 32) {
-                const int qrow = row0 + q;
+            constexpr int kPer = CH / 8;  // pieces of 8 channels per lane
+            float4 all[C::kRows / 32][kPer][2];
+#pragma unroll
+            for (int i = 0; i < C::kRows / 32; ++i) {
+                const int qrow = row0 + i * 32 + (tid >> 3);
                 const bool ok = qrow < P.rows;
                 const int token = (ok ? qrow : 0) / P.group, head = kvh * P.group + (ok ? qrow : 0) % P.group;
                 const float4* qp = reinterpret_cast<const float4*>(P.q + static_cast<size_t>(s) * P.q_seq + static_cast<size_t>(token) * P.q_token + static_cast<size_t>(head) * P.q_head);
-                constexpr int kPer = CH / 8;  // pieces of 8 channels per lane
-                float4 x[kPer][2];
+#pragma unroll
+                for (int k = 0; k < kPer; ++k)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) all[i][k][e] = ok ? qp[2 * (k * 8 + l8) + e] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+#pragma unroll
+            for (int i = 0; i < C::kRows / 32; ++i) {
+                const int q = i * 32 + (tid >> 3);
+                const float4(&x)[kPer][2] = all[i];
                 float amax = 0.0f;
 #pragma unroll
                 for (int k = 0; k < kPer; ++k)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float4 f = ok ? qp[2 * (k * 8 + l8) + e] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        x[k][e] = f;
-                        amax = fmaxf(fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y))), fmaxf(fabsf(f.z), fabsf(f.w)));
-                    }
+                    for (int e = 0; e < 2; ++e) amax = fmaxf(fmaxf(amax, fmaxf(fabsf(x[k][e].x), fabsf(x[k][e].y))), fmaxf(fabsf(x[k][e].z), fabsf(x[k][e].w)));
 #pragma unroll
                 for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
                 float up, down;
@@ -482,7 +487,7 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
         if (GEN) ri = row_info(P, s, kvh, n, row);
         // slots from `limit` on are hidden by the end of the range, or (slot = position) by causality
         int limit = valid ? end : 0;
-        if (P.causal && valid && !(GEN && P.positions)) limit = min(end, max(prefix, row_pos(P, s, n, row / P.group) + 1));
+        if (P.causal && valid && !(GEN && P.positions)) limit = causal_limit(row_pos(P, s, n, row / P.group), prefix, end);
 
         float2 o[D / 4];  // this warpgroup's half of the channels
         float m, l, al;
@@ -557,12 +562,11 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
                         }
                     }
                 } else if (P.bias_step != 0.0f) {
-                    const float qp = static_cast<float>(ri.pos);
                     if (P.positions) {
 #pragma unroll
-                        for (int k = 0; k < HK; ++k) Y(k) -= ri.slope * fabsf(qp - static_cast<float>(meta[k]));
+                        for (int k = 0; k < HK; ++k) Y(k) -= ri.slope * fabsf(static_cast<float>(ri.pos - meta[k]));
                     } else {
-                        const float far = static_cast<float>(ri.pos) - static_cast<float>(t0);
+                        const float far = static_cast<float>(ri.pos - t0);
                         if (__all_sync(0xffffffffu, far >= static_cast<float>(HK - 1))) {  // all of them in front of the query: no absolute value
                             const float nearest = ri.slope * (static_cast<float>(HK - 1) - far);
 #pragma unroll
@@ -704,9 +708,10 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
             else if (P.final_ml) P.final_ml[(static_cast<size_t>(s) * P.kv_heads + kvh) * P.rows + row] = make_float2(m, L);
         }
         named_sync(4, 256);
+#pragma unroll 8
         for (int x = tid; x < C::kRows * (D / 4); x += 256) {
             const int q = x / (D / 4), ch = x % (D / 4) * 4, qrow = row0 + q;
-            if (qrow >= P.rows) break;
+            if (qrow >= P.rows) continue;
             const int token = qrow / P.group, head = kvh * P.group + qrow % P.group;
             float* dst = P.nsplit > 1 ? P.part_o + (part0 + qrow) * D
                                       : P.out + static_cast<size_t>(s) * P.o_seq + static_cast<size_t>(token) * P.o_token + static_cast<size_t>(head) * P.o_head;

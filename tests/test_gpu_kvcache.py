@@ -1,5 +1,8 @@
 """KV-cache operators on the GPU against their 64-bit forms (kv_reference.py)."""
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -311,6 +314,62 @@ def test_offsets_past_32_bits():
         torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("bits", [16, 4])
+def test_long_contexts_keep_their_digits(bits):
+    """Over many keys an output is far smaller than the values it is made of.  Relative to the output's norm: a warp's sums are
+    truncated at most 34 times by at most 2^-23 (4.1e-6; the splits' errors are independent, as their sums are), operands carry
+    22 bits (5e-7), scores move weights by 1.5e-6: below 1e-5."""
+    Hkv, D, cap = 1, 64, 300000
+    c, k, v, gen = filled(bits, 1, cap, Hkv, D, [cap], seed=21)
+    for N in (1, 130):
+        q = torch.randn(1, N, 2, D, generator=gen, device="cuda")
+        out = kvcache.Attention(c, n_tokens=N, heads=2, causal=False)(q).double()
+        want, *_ = ref.attend(q.double(), k, v, c.n_keys, scale=D ** -0.5, causal=False)
+        assert ((out - want).norm() / want.norm()).item() < 1e-5
+
+
+@pytest.mark.parametrize("N", [1, 20, 100])
+def test_query_positions_at_the_ends_of_their_range(N):
+    """The largest position sees everything, the smallest nothing."""
+    c, k, v, gen = filled(16, 1, 90, 1, 64, [90], seed=12)
+    q = torch.randn(1, N, 2, 64, generator=gen, device="cuda")
+    pos = torch.full((1, N), 2 ** 31 - 1, dtype=torch.int32, device="cuda")
+    far = kvcache.Attention(c, n_tokens=N, heads=2, q_pos=pos)(q)
+    assert torch.equal(far, kvcache.Attention(c, n_tokens=N, heads=2, causal=False)(q))
+    pos.fill_(-2 ** 31)
+    assert (kvcache.Attention(c, n_tokens=N, heads=2, q_pos=pos)(q) == 0).all()
+
+
+def test_first_call_inside_a_capture():
+    """A fresh process whose first attention, append and eviction are captured."""
+    code = """
+import torch
+from kernelcore_b200 import kvcache
+torch.cuda.set_device(0)
+c = kvcache.KVCache.empty(1, 2, 64, 300, bits=4, evictable=True)
+k = torch.randn(1, 200, 2, 64, device="cuda")
+q = torch.randn(1, 100, 4, 64, device="cuda")
+att = kvcache.Attention(c, n_tokens=100, heads=4, accumulate=True)
+out = torch.empty_like(q)
+c._evict_ws
+c.evict(299, 1)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    c.append(k, k)
+    att(q, out)
+c.n_keys.zero_(); c.next_pos.zero_()
+g.replay()
+torch.cuda.synchronize()
+first = out.clone()
+c.n_keys.zero_(); c.next_pos.zero_()
+c.append(k, k)
+assert torch.equal(att(q), first) and c.n_keys.tolist() == [200]
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0, r.stderr
+
+
 # ---- eviction -------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("bits", [16, 4])
@@ -419,6 +478,31 @@ def test_a_streaming_decode_loop(bits, graph):
             assert (c.positions[s, :, :cnt[s]].cpu().numpy() == pos[s, :, :cnt[s]]).all()
             assert np.allclose(c.weights[s, :, :cnt[s]].cpu().numpy(), w[s, :, :cnt[s]], rtol=1e-4, atol=1e-7)
             assert (c.read(0, cap)[0][s, :cnt[s]].cpu().numpy() == live[0][s, :cnt[s]].astype(np.float32)).all()
+
+
+@pytest.mark.parametrize("N, H, Hkv, softcap, max_bias", [(3, 6, 2, 30.0, 0.0), (1, 8, 4, 0.0, 8.0), (60, 6, 2, 20.0, 8.0)])
+def test_the_ggml_operator_takes_caps_and_biases(N, H, Hkv, softcap, max_bias):
+    """FLASH_ATTN_EXT with a logit softcap and with ALiBi (slope times the mask, which holds the distances)."""
+    import ctypes as C
+
+    from test_gpu_ggml_ops import F16, F32, f32_bits, op, tensor
+    D, T = 64, 77
+    gen = torch.Generator(device="cuda").manual_seed(N)
+    kc, vc = (torch.randn(T, Hkv, D, generator=gen, device="cuda").half() for _ in range(2))
+    q = torch.randn(H, N, D, generator=gen, device="cuda")                              # ggml's [D, N, H]
+    at = T - N + torch.arange(N, device="cuda").unsqueeze(1)
+    t = torch.arange(80, device="cuda")
+    mask = torch.where((t <= at) & (t < T), -(at - t).abs().float(), -math.inf).half().contiguous()
+    out = torch.zeros(N, H, D, device="cuda")
+    h = C.c_void_p()
+    assert lib.raw.kcb_ggml_ctx_create(None, C.byref(h)) == 0 and lib.raw.kcb_ggml_ctx_begin_graph(h) == 0
+    kt, vt = (tensor(x, F16, [D, T, Hkv], nb=[2, 2 * Hkv * D, 2 * D, 2 * Hkv * D * T]) for x in (kc, vc))
+    params = [f32_bits(0.125), f32_bits(max_bias), f32_bits(softcap)]
+    op("flash_attn", h, tensor(out, F32, [D, H, N], src=(tensor(q, F32, [D, N, H]), kt, vt, tensor(mask, F16, [80, N])), params=params))
+    lib.raw.kcb_ggml_ctx_destroy(h)
+    want, _, tol = ref.attend(q.transpose(0, 1).unsqueeze(0).double(), kc.unsqueeze(0).double(), vc.unsqueeze(0).double(), [T], scale=0.125, softcap=softcap,
+                              max_bias=max_bias, causal=False, mask=mask.unsqueeze(0))
+    assert ((out - want[0]).abs().amax(-1) <= tol[0]).all()
 
 
 def test_two_streams_and_the_same_call_twice():
