@@ -10,6 +10,12 @@ template <>
 int attn_launch<KV_BITS, KV_DIM>(const AttnP& P, bool general, AttnKernel which, cudaStream_t st) {
     return attn_launch_kernels<KV_DIM, KV_BITS>(P, general, which, st);
 }
+#if KV_BITS == 16 && (KV_DIM == 64 || KV_DIM == 128)
+template <>
+int attn_launch_tc_dim<KV_DIM>(const AttnP& P, bool general, cudaStream_t st) {
+    return attn_launch_tc<KV_DIM, 16>(P, general, st);
+}
+#endif
 template <>
 unsigned attn_timeouts_of<KV_BITS, KV_DIM>() {
     return attn_timeouts_here();

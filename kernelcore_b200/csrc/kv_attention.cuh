@@ -46,7 +46,7 @@ struct AttnP {
     const int* k_doc;
     const unsigned short* mask;
     long long mask_token, mask_seq;
-    int cap, n_seqs, n_tokens, heads, kv_heads, group, rows;  // rows = n_tokens * group
+    int dim, cap, n_seqs, n_tokens, heads, kv_heads, group, rows;  // rows = n_tokens * group
     int causal, bias_log2_heads;                      // bias_log2_heads: largest power of two <= heads
     float sc;                                         // score factor: scale * log2 e, or scale / cap with a cap
     float cap_out;                                    // cap * log2 e, 0 without a cap
@@ -1416,7 +1416,9 @@ int attn_launch_rows(const AttnP& P, cudaStream_t st) {
 template <int D, int FMT>
 int attn_launch_kernels(const AttnP& P, bool general, AttnKernel which, cudaStream_t st) {
     if (which == AttnKernel::tc) {
-        int e = attn_launch_tc<D, FMT>(P, general, st);
+        int e = KCB_UNSUPPORTED_OPERATION;
+        if constexpr (FMT == 16 && D <= 128) e = attn_launch_tc_dim<D <= 64 ? 64 : 128>(P, general, st);  // 32 and 96: in the next wider kernel
+        else if constexpr (D == 64 || D == 128) e = attn_launch_tc<D, FMT>(P, general, st);
         if (e == KCB_UNSUPPORTED_OPERATION) {  // strides that a tensor map does not take (sequences that share one cache: stride 0)
             AttnP T = P;
             T.row_tiles = (P.rows + QTile<D>::kRows - 1) / QTile<D>::kRows;

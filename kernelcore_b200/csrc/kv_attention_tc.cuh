@@ -1,5 +1,5 @@
 // Prompt attention over a KV cache on the 5th-generation tensor cores (tcgen05, TMEM): 128 query rows per CTA, head dimension 64 or
-// 128.  Same mathematics and precision as kv_attention.cuh: queries and probabilities as hi + lo fp16 pairs, both multiplied; an fp16
+// 128 (fp16 also 32 and 96, filled up with zeros).  Same mathematics and precision as kv_attention.cuh: queries and probabilities as hi + lo fp16 pairs, both multiplied; an fp16
 // cache exact as it is; 4-bit values d code + m (a multiple of 2^-24, as every fp16 number is) as hi + lo pairs too, of whose four
 // products with a query or probability the smallest, lo * lo (2^-22), is left out.
 //
@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
 #pragma unroll
                 for (int k = 0; k < kPer; ++k)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) all[i][k][e] = ok ? qp[2 * (k * 8 + l8) + e] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (int e = 0; e < 2; ++e) all[i][k][e] = ok && (k * 8 + l8) * 8 < P.dim ? qp[2 * (k * 8 + l8) + e] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             }
 #pragma unroll
             for (int i = 0; i < C::kRows / 32; ++i) {
@@ -669,7 +669,8 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
                         const float p = half_bits_to_float(ph & 0xFFFFu) + half_bits_to_float(pl & 0xFFFFu);
                         if (p != 0.0f)
 #pragma unroll
-                            for (int ch = 0; ch < D / 4; ++ch) add_not_finite(o[ch].x, o[ch].y, p, vp[ch]);
+                            for (int ch = 0; ch < D / 4; ++ch)
+                                if (wg * (D / 2) + 2 * ch < P.dim) add_not_finite(o[ch].x, o[ch].y, p, vp[ch]);
                         __syncwarp();
                     }
                 }
@@ -711,9 +712,9 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
 #pragma unroll 8
         for (int x = tid; x < C::kRows * (D / 4); x += 256) {
             const int q = x / (D / 4), ch = x % (D / 4) * 4, qrow = row0 + q;
-            if (qrow >= P.rows) continue;
+            if (qrow >= P.rows || ch >= P.dim) continue;
             const int token = qrow / P.group, head = kvh * P.group + qrow % P.group;
-            float* dst = P.nsplit > 1 ? P.part_o + (part0 + qrow) * D
+            float* dst = P.nsplit > 1 ? P.part_o + (part0 + qrow) * P.dim
                                       : P.out + static_cast<size_t>(s) * P.o_seq + static_cast<size_t>(token) * P.o_token + static_cast<size_t>(head) * P.o_head;
             *reinterpret_cast<float4*>(dst + ch) = *reinterpret_cast<const float4*>(stage_out + q * kStride + ch);
         }
@@ -763,7 +764,7 @@ int attn_launch_tc(const AttnP& P, bool general, cudaStream_t st) {
     if constexpr (D == 64 || D == 128) {
         using C = TcCfg<D, FMT>;
         CUtensorMap mk{}, mv{};
-        if (FMT == 16 && !(cache_map(&mk, P.k, P, D, P.k_row, P.k_head, P.k_seq, C::KT) && cache_map(&mv, P.v, P, D, P.v_row, P.v_head, P.v_seq, C::KT)))
+        if (FMT == 16 && !(cache_map(&mk, P.k, P, P.dim, P.k_row, P.k_head, P.k_seq, C::KT) && cache_map(&mv, P.v, P, P.dim, P.v_row, P.v_head, P.v_seq, C::KT)))
             return KCB_UNSUPPORTED_OPERATION;
         static PerDeviceFlag raised[2];
         const dim3 grid(P.row_tiles * P.nsplit, P.kv_heads, P.n_seqs);

@@ -201,7 +201,6 @@ __global__ void __launch_bounds__(kRowThreads) kv_read_rows_kernel(const __grid_
 // from the lowest slot on.  Then the free slots below `keep` and the kept rows at or behind it are listed in ascending order: the
 // j-th kept row moves into the j-th free slot, so sources and destinations are disjoint and the rows can move in place, in
 // parallel and in any order (the positions beside them say where a row belongs).
-constexpr int kSelThreads = 1024;
 constexpr int kSelKeys = 50 * 1024;  // keys kept in shared memory; longer caches compute them anew in every pass
 
 struct EvictP {
@@ -224,21 +223,22 @@ __device__ __forceinline__ int warp_prefix(int v, int* slots, int& total) {
     if (lane == 0) slots[warp] = v;
     __syncthreads();
     if (warp == 0) {
-        const int t = slots[lane];
+        const int t = lane < static_cast<int>(blockDim.x >> 5) ? slots[lane] : 0;
         int y = t;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int z = __shfl_up_sync(0xffffffffu, y, o);
             if (lane >= o) y += z;
         }
-        slots[lane] = y - t;
+        if (lane < static_cast<int>(blockDim.x >> 5)) slots[lane] = y - t;
         if (lane == 31) slots[32] = y;
     }
     __syncthreads();
     total = slots[32];
     return slots[warp];
 }
-__global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_constant__ EvictP E) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) kv_select_kernel(const __grid_constant__ EvictP E) {
     extern __shared__ unsigned keys[];
     __shared__ int hist[2048], slots[33], digit, rest;
     const kcb_kv_cache& c = E.c;
@@ -263,10 +263,11 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_con
 #pragma unroll 1
     for (int round = 0; round < 3; ++round) {
         const int shift = round == 0 ? 21 : round == 1 ? 10 : 0, bins = round < 2 ? 2048 : 1024;
-        hist[tid] = 0, hist[tid + 1024] = 0;
+#pragma unroll
+        for (int i = 0; i < 2048 / THREADS; ++i) hist[i * THREADS + tid] = 0;
         __syncthreads();
-#pragma unroll 4
-        for (int t = tid; t < n; t += kSelThreads) {
+#pragma unroll 8
+        for (int t = tid; t < n; t += THREADS) {
             unsigned k;
             if (round == 0) {
                 k = make_key(t);
@@ -277,19 +278,27 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_con
             if ((k & mask) == prefix) atomicAdd(&hist[k >> shift & (bins - 1)], 1);
         }
         __syncthreads();
-        // from the largest digit down, two to a thread: where does the need-th key fall?
-        const int a = bins - 1 - 2 * tid, ha = a > 0 ? hist[a] : 0, hb = a > 0 ? hist[a - 1] : 0;
-        int before = ha + hb;
+        // from the largest digit down, neighbouring ones to a thread: where does the need-th key fall?
+        constexpr int kMine = 2048 / THREADS;
+        const int a = bins - 1 - kMine * tid;
+        int h[kMine], sum = 0;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) sum += h[i] = a - i >= 0 ? hist[a - i] : 0;
+        int before = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int y = __shfl_up_sync(0xffffffffu, before, o);
             if (lane >= o) before += y;
         }
         int all;
-        before += warp_prefix(__shfl_sync(0xffffffffu, before, 31), slots, all) - (ha + hb);
-        if (before < need && need <= before + ha + hb) {
-            const bool first = need - before <= ha;
-            digit = first ? a : a - 1, rest = need - before - (first ? 0 : ha);
+        before += warp_prefix(__shfl_sync(0xffffffffu, before, 31), slots, all) - sum;
+        if (before < need && need <= before + sum) {
+            int left = need - before;
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+                if (left > 0 && left <= h[i]) digit = a - i, rest = left;
+                left -= h[i];
+            }
         }
         __syncthreads();
         prefix |= static_cast<unsigned>(digit) << shift;
@@ -299,7 +308,8 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_con
     }
     // prefix: the keep-th largest key; `need` rows that equal it stay.  Each warp looks after a run of neighbouring slots, 32 at a
     // time, so that ballots give the ascending order.
-    const int run = ((n + 31) / 32 + 31) / 32 * 32, t0 = min(n, warp * run), t1 = min(n, t0 + run);
+    constexpr int kWarps = THREADS / 32;
+    const int run = ((n + kWarps - 1) / kWarps + 31) / 32 * 32, t0 = min(n, warp * run), t1 = min(n, t0 + run);
     const unsigned below = (1u << lane) - 1u;
     int ties = 0, total;
     for (int t = t0; t < t1; t += 32) ties += __popc(__ballot_sync(0xffffffffu, t + lane < t1 && key_of(t + lane) == prefix));
@@ -423,10 +433,12 @@ struct AttnCut {
     size_t bytes() const { return ml_bytes + o_bytes + final_bytes + score_bytes; }
 };
 constexpr int kTcRows = 96;  // query rows per kv head from which the tcgen05 kernel is taken
+// fp16 rows of 32 and 96 channels go through the kernels for 64 and 128, filled up with zeros by the tensor copies.
+bool tc_takes(const kcb_kv_cache* c) { return c->bits == KCB_CACHE_F16 ? c->head_dim <= 128 : c->head_dim == 64 || c->head_dim == 128; }
 AttnCut attn_cut(const kcb_kv_cache* c, const kcb_cache_attn* a) {
     AttnCut r{};
     const long long rows = static_cast<long long>(a->n_tokens) * (a->heads / c->kv_heads);
-    r.which = rows <= kRowsMax ? AttnKernel::rows : rows >= kTcRows && (c->head_dim == 64 || c->head_dim == 128) ? AttnKernel::tc : AttnKernel::tile;
+    r.which = rows <= kRowsMax ? AttnKernel::rows : rows >= kTcRows && tc_takes(c) ? AttnKernel::tc : AttnKernel::tile;
     const int per = r.which == AttnKernel::rows ? 8 : r.which == AttnKernel::tile ? 64 : 128;
     r.row_tiles = static_cast<int>((rows + per - 1) / per);
     const long long ctas = static_cast<long long>(c->n_seqs) * c->kv_heads * r.row_tiles;
@@ -534,8 +546,12 @@ int kcb_cache_evict(const kcb_kv_cache* c, int keep, int recent, void* workspace
              reinterpret_cast<int2*>(static_cast<uint8_t*>(workspace) + moves_offset(c)), static_cast<long long>(q4_seq_bytes(c->kv_heads, c->head_dim, c->capacity)),
              static_cast<long long>(q4_param_offset(c->kv_heads, c->head_dim, c->capacity))};
     static PerDeviceFlag raised;
-    if (!raise_dynamic_smem(kv_select_kernel, kSelKeys * 4, raised)) return KCB_LAUNCH_FAILURE;
-    kv_select_kernel<<<dim3(c->kv_heads, c->n_seqs), kSelThreads, std::min(c->capacity, kSelKeys) * 4, st>>>(E);
+    if (!raise_dynamic_smem(kv_select_kernel<1024>, kSelKeys * 4, raised)) return KCB_LAUNCH_FAILURE;
+    const dim3 heads(c->kv_heads, c->n_seqs);
+    const size_t smem = static_cast<size_t>(std::min(c->capacity, kSelKeys)) * 4;
+    // short caches in small CTAs, whose barriers are cheaper
+    if (c->capacity <= 4096) kv_select_kernel<256><<<heads, 256, smem, st>>>(E);
+    else kv_select_kernel<1024><<<heads, 1024, smem, st>>>(E);
     if (const int e = launch_status(); e != KCB_SUCCESS) return e;
     constexpr int per_cta = kMoveWarps * kMoveRows;
     const dim3 grid(std::min((E.max_moves + per_cta - 1) / per_cta, 1024), c->kv_heads, c->n_seqs);
@@ -567,7 +583,7 @@ int kcb_cache_attention(const kcb_kv_cache* c, const kcb_cache_attn* a, const fl
     P.n_keys = c->n_keys, P.next_pos = c->next_pos, P.positions = c->positions, P.weights = c->weights;
     P.prefix = a->prefix, P.q_pos = a->q_pos, P.q_doc = a->q_doc, P.k_doc = a->k_doc;
     P.mask = static_cast<const unsigned short*>(a->mask), P.mask_token = a->mask_token, P.mask_seq = a->mask_seq;
-    P.cap = c->capacity, P.n_seqs = c->n_seqs, P.n_tokens = a->n_tokens, P.heads = a->heads, P.kv_heads = c->kv_heads;
+    P.dim = c->head_dim, P.cap = c->capacity, P.n_seqs = c->n_seqs, P.n_tokens = a->n_tokens, P.heads = a->heads, P.kv_heads = c->kv_heads;
     P.group = a->heads / c->kv_heads, P.rows = a->n_tokens * P.group;
     P.causal = a->causal != 0;
     P.bias_log2_heads = 1;

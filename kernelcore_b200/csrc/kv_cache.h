@@ -16,6 +16,9 @@ struct AttnP;
 enum class AttnKernel { rows, tile, tc };
 template <int BITS, int D>
 int attn_launch(const AttnP& P, bool general, AttnKernel which, cudaStream_t st);
+// The tcgen05 kernel for fp16 caches, built for 64 and 128 channels; P.dim may be smaller (the rest is zeros).
+template <int D>
+int attn_launch_tc_dim(const AttnP& P, bool general, cudaStream_t st);
 template <int BITS, int D>
 unsigned attn_timeouts_of();
 int attn_launch_bits(const AttnP& P, int bits, int head_dim, bool general, AttnKernel which, cudaStream_t st);
