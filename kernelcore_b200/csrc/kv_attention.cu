@@ -16,10 +16,12 @@ int attn_launch_tc_dim<KV_DIM>(const AttnP& P, bool general, cudaStream_t st) {
     return attn_launch_tc<KV_DIM, 16>(P, general, st);
 }
 #endif
+#if KV_DIM == 64 || KV_DIM == 128
 template <>
 unsigned attn_timeouts_of<KV_BITS, KV_DIM>() {
     return attn_timeouts_here();
 }
+#endif
 }  // namespace kcb
 
 #else

@@ -25,7 +25,7 @@ namespace kcb {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kPShift = 12.0f;  // probabilities enter the products times 2^12
-constexpr int kRowsMax = 16;      // a rows launch takes at most this many query rows per kv head; more go to a tile launch
+constexpr int kRowsMax = 32;      // a rows launch takes at most this many query rows per kv head (the join keeps that many sums)
 
 // Everything a launch needs, by value.  Strides are in elements (halves, floats).
 struct AttnP {
@@ -798,10 +798,51 @@ __global__ void __launch_bounds__(32 * kRowsWarps, FMT == 16 && D == 128 ? 2 : 1
 }
 
 // ---- joining the splits of a row -------------------------------------------------------------------------------------------
-// One CTA per row: its warps take the splits in turn, then the warps' sums are joined through shared memory.
+// By warps (at most 32 splits): one warp per row, eight splits of it in flight.  Else one CTA per row, whose warps take the splits in
+// turn and join their sums through shared memory.  Warps where there are at most as many splits as a CTA has warps (8192 rows in two
+// splits 3 us, by CTAs 20), or more rows than the GPU holds CTAs of (2048 rows in 9 or 18 splits: the call 26.7 and 28.7 us, by CTAs 30.8
+// and 32.8); else CTAs (384 rows in 18 splits: 22.5, by warps 24.6).
+constexpr int kMergeWarps = 8;
+__device__ __forceinline__ float4* merged_row(const AttnP& P, int s, int kvh, int r) {
+    return reinterpret_cast<float4*>(P.out + static_cast<size_t>(s) * P.o_seq + static_cast<size_t>(r / P.group) * P.o_token + static_cast<size_t>(kvh * P.group + r % P.group) * P.o_head);
+}
+template <int D>
+__global__ void __launch_bounds__(32 * kMergeWarps) attn_merge_warps_kernel(const __grid_constant__ AttnP P) {
+    constexpr int W = kMergeWarps, Q = (D / 4 + 31) / 32;
+    grid_dependency_wait();
+    const int lane = threadIdx.x & 31, kvh = blockIdx.y, s = blockIdx.z;
+    const int r = blockIdx.x * W + (threadIdx.x >> 5);
+    if (r >= P.rows) return;
+    const size_t base = (static_cast<size_t>(s) * P.kv_heads + kvh) * P.nsplit;
+    const float2 t = lane < P.nsplit ? P.part_ml[(base + lane) * P.rows + r] : make_float2(0.0f, 0.0f);
+    const float M = warp_max(t.y != 0.0f ? t.x : -INFINITY), f = t.y != 0.0f ? ex2(t.x - M) : 0.0f, L = warp_sum(t.y != 0.0f ? f * t.y : 0.0f);
+    const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;
+    float4* out = merged_row(P, s, kvh, r);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        const int x = q * 32 + lane;
+        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+        for (int i0 = 0; i0 < P.nsplit; i0 += W) {
+            float4 v[W];
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+                if (i0 + i < P.nsplit && x < D / 4) v[i] = reinterpret_cast<const float4*>(P.part_o + ((base + i0 + i) * P.rows + r) * D)[x];
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                const float fi = __shfl_sync(0xffffffffu, f, i0 + i), ly = __shfl_sync(0xffffffffu, t.y, i0 + i);
+                if (ly != 0.0f && x < D / 4)  // a split in which the row saw nothing has no sums
+                    a.x = fmaf(fi, v[i].x, a.x), a.y = fmaf(fi, v[i].y, a.y), a.z = fmaf(fi, v[i].z, a.z), a.w = fmaf(fi, v[i].w, a.w);
+            }
+        }
+        if (x < D / 4) out[x] = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+    }
+    if (P.final_ml && lane == 0) P.final_ml[(static_cast<size_t>(s) * P.kv_heads + kvh) * P.rows + r] = make_float2(M, L);
+}
+
 // After a rows launch that also wants weights, further CTAs (blockIdx.x from `joins` on) turn 2048 slots' scores into weights each:
 // weights[t] += sum over the rows of 2^(score - M) / L, the rows in order, no atomics.
-constexpr int kWeightSlots = 2048, kMergeWarps = 8;
+constexpr int kWeightSlots = 2048;
 template <int D>
 __global__ void __launch_bounds__(32 * kMergeWarps) attn_merge_kernel(const __grid_constant__ AttnP P, int joins) {
     constexpr int W = kMergeWarps, Q = (D / 4 + 31) / 32;
@@ -886,8 +927,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) attn_merge_kernel(const __gr
 #pragma unroll
     for (int w = 0; w < W; ++w) L += ml[w].y;
     const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;
-    const int tok = row / P.group, head = kvh * P.group + row % P.group;
-    float* out = P.out + static_cast<size_t>(s) * P.o_seq + static_cast<size_t>(tok) * P.o_token + static_cast<size_t>(head) * P.o_head;
+    float4* out = merged_row(P, s, kvh, row);
     for (int x = threadIdx.x; x < D / 4; x += 32 * W) {
         float4 r = acc[0][x];
 #pragma unroll
@@ -895,7 +935,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) attn_merge_kernel(const __gr
             const float4 v = acc[w][x];
             r.x += v.x, r.y += v.y, r.z += v.z, r.w += v.w;
         }
-        reinterpret_cast<float4*>(out)[x] = make_float4(r.x * inv, r.y * inv, r.z * inv, r.w * inv);
+        out[x] = make_float4(r.x * inv, r.y * inv, r.z * inv, r.w * inv);
     }
     if (P.final_ml && threadIdx.x == 0) P.final_ml[(static_cast<size_t>(s) * P.kv_heads + kvh) * P.rows + row] = make_float2(M, L);
 }
@@ -1391,18 +1431,13 @@ __global__ void __launch_bounds__(128) attn_weights_kernel(const __grid_constant
 template <int D, int FMT>
 int attn_launch_tc(const AttnP& P, bool general, cudaStream_t st);
 
-template <int D, int FMT>
-int attn_launch_tile(const AttnP& P, bool general, cudaStream_t st) {
+template <int D, int FMT, bool GEN>
+int attn_launch_tile(const AttnP& P, cudaStream_t st) {
     constexpr int smem = TileCfg<D, FMT>::kSmem;
-    static PerDeviceFlag raised[2];
+    static PerDeviceFlag raised;
     const dim3 grid(P.row_tiles * P.nsplit, P.kv_heads, P.n_seqs);
-    if (general) {
-        if (!raise_dynamic_smem(attn_tile_kernel<D, FMT, true>, smem, raised[0])) return KCB_LAUNCH_FAILURE;
-        attn_tile_kernel<D, FMT, true><<<grid, 128, smem, st>>>(P);
-    } else {
-        if (!raise_dynamic_smem(attn_tile_kernel<D, FMT, false>, smem, raised[1])) return KCB_LAUNCH_FAILURE;
-        attn_tile_kernel<D, FMT, false><<<grid, 128, smem, st>>>(P);
-    }
+    if (!raise_dynamic_smem(attn_tile_kernel<D, FMT, GEN>, smem, raised)) return KCB_LAUNCH_FAILURE;
+    attn_tile_kernel<D, FMT, GEN><<<grid, 128, smem, st>>>(P);
     return launch_status();
 }
 template <int D, int FMT, int MODE>
@@ -1419,14 +1454,18 @@ int attn_launch_kernels(const AttnP& P, bool general, AttnKernel which, cudaStre
         int e = KCB_UNSUPPORTED_OPERATION;
         if constexpr (FMT == 16 && D <= 128) e = attn_launch_tc_dim<D <= 64 ? 64 : 128>(P, general, st);  // 32 and 96: in the next wider kernel
         else if constexpr (D == 64 || D == 128) e = attn_launch_tc<D, FMT>(P, general, st);
-        if (e == KCB_UNSUPPORTED_OPERATION) {  // strides that a tensor map does not take (sequences that share one cache: stride 0)
-            AttnP T = P;
-            T.row_tiles = (P.rows + QTile<D>::kRows - 1) / QTile<D>::kRows;
-            e = attn_launch_tile<D, FMT>(T, true, st);
-        }
+        if constexpr (FMT == 16 && D <= 128)
+            if (e == KCB_UNSUPPORTED_OPERATION) {  // strides that a tensor map does not take (sequences that share one cache: stride 0)
+                AttnP T = P;
+                T.row_tiles = (P.rows + QTile<D>::kRows - 1) / QTile<D>::kRows;
+                e = attn_launch_tile<D, FMT, true>(T, st);
+            }
         if (e != KCB_SUCCESS) return e;
     } else if (which == AttnKernel::tile) {
-        if (const int e = attn_launch_tile<D, FMT>(P, general, st); e != KCB_SUCCESS) return e;
+        int e = KCB_UNSUPPORTED_OPERATION;
+        if constexpr (D == 256 || (FMT == 4 && D != 64 && D != 128))  // the shapes that tcgen05 does not take
+            e = general ? attn_launch_tile<D, FMT, true>(P, st) : attn_launch_tile<D, FMT, false>(P, st);
+        if (e != KCB_SUCCESS) return e;
     } else {
         int e;
         if (P.positions || P.q_doc || P.mask) e = attn_launch_rows<D, FMT, 2>(P, st);
@@ -1434,8 +1473,12 @@ int attn_launch_kernels(const AttnP& P, bool general, AttnKernel which, cudaStre
         else e = attn_launch_rows<D, FMT, 0>(P, st);
         if (e != KCB_SUCCESS) return e;
     }
-    const int joins = P.nsplit > 1 ? P.rows : 0, weights = P.scores ? (P.cap + kWeightSlots - 1) / kWeightSlots : 0;
-    if (joins + weights) {
+    const bool by_warps = P.nsplit <= kMergeWarps || (P.nsplit <= 32 && static_cast<long long>(P.rows) * P.kv_heads * P.n_seqs > 8 * kSmCount);
+    if (P.nsplit > 1 && by_warps && !P.scores) {
+        const int e = launch_dependent(attn_merge_warps_kernel<D>, dim3((P.rows + kMergeWarps - 1) / kMergeWarps, P.kv_heads, P.n_seqs), 32 * kMergeWarps, 0, st, P);
+        if (e != KCB_SUCCESS) return e;
+    } else if (P.nsplit > 1 || P.scores) {
+        const int joins = P.nsplit > 1 ? P.rows : 0, weights = P.scores ? (P.cap + kWeightSlots - 1) / kWeightSlots : 0;
         const int e = launch_dependent(attn_merge_kernel<D>, dim3(joins + weights, P.kv_heads, P.n_seqs), 32 * kMergeWarps, 0, st, P, joins);
         if (e != KCB_SUCCESS) return e;
     }

@@ -42,8 +42,8 @@ struct TcCfg {
     static constexpr int kStages = kSlot > 16384 ? 2 : 4;      // of keys, and of values
     static constexpr int kQHalf = kRows * D * 2;               // hi, then lo queries
     static constexpr int kOffK = 2 * kQHalf, kOffV = kOffK + kStages * kSlot;
-    static constexpr int kMeta = kOffV + kStages * kSlot;      // per stage: KT positions, KT documents, 16 bytes free, bits of odd slots
-    static constexpr int kMetaBytes = 2 * KT * 4 + 32;
+    static constexpr int kMeta = kOffV + kStages * kSlot;      // per stage: KT positions, KT documents, bits of odd slots
+    static constexpr int kMetaBytes = 2 * KT * 4 + 16;
     static constexpr int kMax = kMeta + kStages * kMetaBytes;  // maxima exchanged: [2][warpgroup][row]
     static constexpr int kBars = kMax + 2 * 2 * kRows * 4;
     static constexpr int kTile0 = kBars + 256;                 // bitmap of tiles
@@ -385,7 +385,6 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
                 }
             } else {
                 for (bool careful = false;; careful = true) {
-                    const int i0 = i;
                     for (int tile = next(-1); tile < nt; tile = next(tile), ++i) {
                         const int st = i % C::kStages, ph = (i / C::kStages - 1) & 1, t0 = begin + tile * KT;
                         uint8_t* vt = sm + C::kOffV + st * C::kSlot;
@@ -406,7 +405,7 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
                         }
                         if (careful) {
                             __syncwarp();
-                            unsigned* odd = reinterpret_cast<unsigned*>(sm + C::kMeta + st * C::kMetaBytes + 2 * KT * 4 + 16);
+                            unsigned* odd = reinterpret_cast<unsigned*>(sm + C::kMeta + st * C::kMetaBytes + 2 * KT * 4);
                             tc_wait(&varrived[st], (i / C::kStages) & 1, fail);
                             if (ptid < KT / 32) odd[ptid] = 0u;
                             named_sync(3, C::kProducers);  // nobody sets a bit before they are cleared
@@ -649,7 +648,7 @@ __global__ void __launch_bounds__(TcCfg<D, FMT>::kThreads, 1)
             tc_st_wait();
             if (FMT == 16 && careful) {  // values of this tile that are not finite go to the rows that see them one by one
                 tc_wait(&vfull[st], ((i - i0) / C::kStages) & 1, fail);
-                const unsigned* odd = reinterpret_cast<const unsigned*>(sm + C::kMeta + st * C::kMetaBytes + 2 * KT * 4 + 16);
+                const unsigned* odd = reinterpret_cast<const unsigned*>(sm + C::kMeta + st * C::kMetaBytes + 2 * KT * 4);
                 unsigned any = 0;
 #pragma unroll
                 for (int h = 0; h < KT / 32; ++h) any |= odd[h];

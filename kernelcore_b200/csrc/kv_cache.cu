@@ -432,17 +432,37 @@ struct AttnCut {
     size_t ml_bytes, o_bytes, final_bytes, score_bytes;
     size_t bytes() const { return ml_bytes + o_bytes + final_bytes + score_bytes; }
 };
-constexpr int kTcRows = 96;  // query rows per kv head from which the tcgen05 kernel is taken
-// fp16 rows of 32 and 96 channels go through the kernels for 64 and 128, filled up with zeros by the tensor copies.
+// The tcgen05 kernel takes fp16 rows of 32 and 96 channels too, filled up with zeros to 64 and 128 by the tensor copies.
 bool tc_takes(const kcb_kv_cache* c) { return c->bits == KCB_CACHE_F16 ? c->head_dim <= 128 : c->head_dim == 64 || c->head_dim == 128; }
+// Which kernel (us on a B200, 32 query heads over 8, D = 128 unless said).  The rows kernel reads the cache once per 8 query rows of a
+// kv head, straight into registers; the other two once per 64 or 128, through shared memory.
+//   fp16, 8 rows: rows 45, tcgen05 47 (32768 slots), 129 and 137 (32 sequences of 4096).  16 rows: the long caches favour tcgen05 (59 and
+//   47, 221 and 137), the short ones rows (512 slots: 12 and 18, 4096: 20.5 and 21.7); they meet near 2^17 slots over all heads and
+//   sequences (D = 64: 25.8 and 31.6, D = 96: 35.8 and 33.8).  24 rows: 86 and 47.  With weights rows lead up to 16 (16 sequences of
+//   4096: 206 and 208), for they keep the scores, where the others compute them anew.
+//   4 bits, whose unpacking costs the tile kernels more than reading twice costs rows: 32 rows 67 and 83 (32768 slots), 237 and 305 (32
+//   sequences); D = 64: 79 and 123, and 40 rows 95 and 123.
+//   Where tcgen05 does not take a shape, rows and tiles: fp16, D = 256, 16 rows 302 and 437, 20 rows 439 and 439; 4 bits, D = 256, 20
+//   rows 386 and 427, but 101 and 119 is no more than a fourth group of rows would cost.  The tile kernel never leads tcgen05 by more
+//   than a tenth (4 bits, D = 64, up to 64 rows: 38 and 42), and loses by two to three from 96 rows on.
+AttnKernel attn_kernel(const kcb_kv_cache* c, const kcb_cache_attn* a, long long rows) {
+    const long long slots = static_cast<long long>(c->n_seqs) * c->kv_heads * c->capacity;
+    long long few = kRowsMax / 2;
+    if (c->bits == KCB_CACHE_Q4 && tc_takes(c)) few = kRowsMax;
+    else if (tc_takes(c) && !a->accumulate && slots > 1 << 17) few = 8;
+    return rows <= few ? AttnKernel::rows : tc_takes(c) ? AttnKernel::tc : AttnKernel::tile;
+}
 AttnCut attn_cut(const kcb_kv_cache* c, const kcb_cache_attn* a) {
     AttnCut r{};
     const long long rows = static_cast<long long>(a->n_tokens) * (a->heads / c->kv_heads);
-    r.which = rows <= kRowsMax ? AttnKernel::rows : rows >= kTcRows && tc_takes(c) ? AttnKernel::tc : AttnKernel::tile;
+    r.which = attn_kernel(c, a, rows);
     const int per = r.which == AttnKernel::rows ? 8 : r.which == AttnKernel::tile ? 64 : 128;
     r.row_tiles = static_cast<int>((rows + per - 1) / per);
     const long long ctas = static_cast<long long>(c->n_seqs) * c->kv_heads * r.row_tiles;
-    const long long want = (r.which == AttnKernel::rows ? (c->n_seqs == 1 ? 2 : 4) : r.which == AttnKernel::tile ? 2 : 1) * kSmCount, least = r.which == AttnKernel::rows ? 128 : 512;
+    // Keys are split until the GPU is full, one CTA per SM (tcgen05; 4 bits, 256 rows of 16384 slots: 86 us, with twice as many 96) or
+    // two (rows and tiles; 64 rows of 16384: 47, with one 57), but into no fewer than 128 slots (12 rows of 512 slots: tcgen05 15, with
+    // 512 slots a split 20; tiles 17 and 31; 64 slots gain nothing).
+    const long long want = (r.which == AttnKernel::tc ? 1 : 2) * kSmCount, least = 128;
     r.nsplit = static_cast<int>(std::max<long long>(1, std::min<long long>(want / std::max<long long>(ctas, 1), (c->capacity + least - 1) / least)));
     // A rows launch adds values up on the tensor cores, whose sums truncate: at most 2048 slots per split are 32 additions per warp
     // (131072 4-bit rows, relative error against 64 bits: 6.4e-6 with 3543 slots a split, 2.8e-6 with 1771).  More splits than the
@@ -505,7 +525,9 @@ int kcb_cache_append(const kcb_kv_cache* c, const float* k, const float* v, int 
     if (n_tokens == 0 || c->n_seqs == 0) return KCB_SUCCESS;
     const auto st = static_cast<cudaStream_t>(stream);
     const unsigned blocks = row_blocks(c, n_tokens);
-    const bool one = blocks <= 4;  // a step's few rows: one CTA per sequence, which also moves the counts on
+    // a step's few rows: one CTA per sequence, which also moves the counts on (6.2 us, in two launches 8.2; from two CTAs' rows on 10.2
+    // and 8.2)
+    const bool one = blocks == 1;
     AppendP A{*c, k, v, token_stride, seq_stride, static_cast<long long>(q4_seq_bytes(c->kv_heads, c->head_dim, c->capacity)),
               static_cast<long long>(q4_param_offset(c->kv_heads, c->head_dim, c->capacity)), divisor(c->kv_heads), n_tokens, one};
     const dim3 grid(one ? 1 : blocks, c->n_seqs);
@@ -549,8 +571,9 @@ int kcb_cache_evict(const kcb_kv_cache* c, int keep, int recent, void* workspace
     if (!raise_dynamic_smem(kv_select_kernel<1024>, kSelKeys * 4, raised)) return KCB_LAUNCH_FAILURE;
     const dim3 heads(c->kv_heads, c->n_seqs);
     const size_t smem = static_cast<size_t>(std::min(c->capacity, kSelKeys)) * 4;
-    // short caches in small CTAs, whose barriers are cheaper
-    if (c->capacity <= 4096) kv_select_kernel<256><<<heads, 256, smem, st>>>(E);
+    // Many short caches in small CTAs, of which an SM holds more (64 sequences of 8 heads: 576 slots 23.6 us, with 1024 threads 27.6; 2048
+    // slots 69 and 75, 4096 slots 83 and 79); where every CTA has an SM the wider one is as fast or faster (4 sequences of 2048: 21 and 24).
+    if (c->capacity <= 2048 && heads.x * heads.y > kSmCount) kv_select_kernel<256><<<heads, 256, smem, st>>>(E);
     else kv_select_kernel<1024><<<heads, 1024, smem, st>>>(E);
     if (const int e = launch_status(); e != KCB_SUCCESS) return e;
     constexpr int per_cta = kMoveWarps * kMoveRows;

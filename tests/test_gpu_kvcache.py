@@ -128,7 +128,7 @@ SHAPES = [  # S, N, heads, kv heads, D, capacity, rows in use
     (1, 1, 16, 1, 256, 50, [33]), (1, 2, 32, 8, 128, 1000, [999]), (2, 5, 3, 3, 32, 40, [40, 3]), (1, 1, 24, 1, 64, 700, [700]),
     (1, 17, 4, 4, 128, 64, [64]), (2, 33, 8, 2, 64, 130, [129, 40]), (1, 65, 2, 1, 96, 65, [65]), (1, 40, 6, 2, 256, 100, [90]), (1, 130, 5, 1, 32, 300, [290]),
     (1, 100, 8, 8, 128, 1300, [1222]), (1, 16, 8, 4, 64, 5000, [4801]),
-    # 96 rows per kv head and more at D = 64 and 128: the tcgen05 kernel (one row tile and several, one key tile, few, many, split)
+    # the tcgen05 kernel: one row tile and several, one key tile, few, many, split
     (1, 96, 1, 1, 64, 96, [96]), (1, 97, 3, 3, 128, 97, [97]), (2, 130, 4, 2, 128, 150, [150, 131]), (1, 300, 6, 2, 64, 700, [650]), (1, 128, 1, 1, 128, 3000, [2999]),
     (3, 64, 4, 2, 64, 64, [64, 0, 1]), (1, 1000, 2, 2, 128, 1000, [1000]), (1, 50, 16, 2, 128, 63, [63])]
 
@@ -141,6 +141,20 @@ def test_attention_shapes(bits, shape):
     q = torch.randn(S, N, H, D, generator=gen, device="cuda")
     check(c, k, v, q, N, H)
     check(c, k, v, q, N, H, causal=False)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("weights", [False, True], ids=["", "weights"])
+@pytest.mark.parametrize("rows, Hkv, D, cap", [(8, 1, 64, 500), (9, 1, 128, 500), (15, 2, 64, 300), (16, 1, 128, 2100), (17, 2, 128, 300), (32, 2, 64, 333), (32, 1, 128, 2500),
+                                               (33, 1, 128, 300), (9, 4, 32, 33000), (16, 4, 64, 33000), (24, 1, 256, 300), (17, 1, 96, 200)])
+def test_attention_at_the_rows_where_kernels_change(bits, weights, rows, Hkv, D, cap):
+    """Query rows of a kv head, as tokens times grouped heads, around every limit of the choice; 2^17 slots are one of them."""
+    group = 4 if rows % 4 == 0 else 3 if rows % 3 == 0 else 1
+    N, H = rows // group, group * Hkv
+    c, k, v, gen = filled(bits, 1, cap, Hkv, D, [cap - 3], seed=rows + D, evictable=weights)
+    q = torch.randn(1, N, H, D, generator=gen, device="cuda")
+    check(c, k, v, q, N, H, accumulate=weights)
+    check(c, k, v, q, N, H, accumulate=weights, softcap=8.0, max_bias=2.0)
 
 
 FORMS = ["cap", "bias", "cap bias", "prefix", "docs", "mask", "mask slopes", "positions", "weights", "all"]
@@ -188,7 +202,7 @@ def test_attention_forms(bits, N, H, Hkv, D, cap, form):
 @pytest.mark.parametrize("N", [1, 24, 150])
 def test_attention_of_small_and_large_values(bits, size, N):
     """Values (and, scaled back, keys) of every magnitude that fp16 holds: the probabilities' split must not lose them."""
-    c, k, v, gen = filled(bits, 1, 200, 2, 64, [200], seed=11, size=size)   # (96 rows and more: the tcgen05 kernel)
+    c, k, v, gen = filled(bits, 1, 200, 2, 64, [200], seed=11, size=size)
     q = torch.randn(1, N, 4, 64, generator=gen, device="cuda")
     check(c, k, v, q, N, 4, scale=0.125 / size)
     check(c, k, v, 1e-6 * q, N, 4, scale=1e6 * 0.125 / size)
