@@ -307,7 +307,8 @@ typedef struct {
 size_t kcb_cache_bytes(int bits, int n_seqs, int kv_heads, int head_dim, int capacity);
 /* n_tokens new rows per sequence behind the n_keys in use: fp32 [kv_heads][head_dim] at k + seq * seq_stride + token *
  * token_stride floats (multiples of 4; k and v 16-byte aligned).  Then n_keys and next_pos grow by n_tokens; the rows'
- * positions are next_pos + token, their weights 0.  Rows beyond the capacity are dropped and n_keys stops there. */
+ * positions are next_pos + token, their weights 0.  Rows beyond the capacity are dropped and n_keys stops there.  An fp16 cache whose
+ * sequences, heads or slots share rows (stride 0) can be attended to but not written: InvalidValue, here and in kcb_cache_evict. */
 int kcb_cache_append(const kcb_kv_cache* cache, const float* k_dev, const float* v_dev, int n_tokens, int64_t token_stride, int64_t seq_stride,
                   void* stream);
 /* Slots first .. first + count - 1 of every sequence as fp32 [n_seqs][count][kv_heads][head_dim], the values that the
@@ -317,7 +318,8 @@ int kcb_cache_read(const kcb_kv_cache* cache, int first, int count, float* k_out
 /* Attention of n_tokens query tokens per sequence over the cache.  Scores are scale * q.k; softcap > 0 bends them to
  * softcap * tanh(score / softcap); max_bias > 0 gives every head the slope 2^-(max_bias (h + 1) / H) (H: the largest power
  * of two of heads; the heads behind it 2^-(max_bias (2 (h - H) + 1) / 2H)) and subtracts slope * |query position - key
- * position|, or, with an additive mask, adds slope * mask instead of the mask (ggml's convention).
+ * position|, or, with an additive mask, adds slope * mask instead of the mask (ggml's convention).  |scale| / softcap must lie
+ * between 1e-20 and 1e20.
  * A query sees a slot that is in use and that nothing hides:
  *   causal != 0    the key's position is at most the query's, or below prefix[seq] (prefix may be NULL)
  *   q_doc, k_doc   the document of the query [n_seqs][n_tokens] equals that of the slot [n_seqs][capacity]
@@ -327,7 +329,7 @@ int kcb_cache_read(const kcb_kv_cache* cache, int first, int count, float* k_out
  * Documents and masks go by slot, so a cache with positions refuses them (InvalidValue).
  * accumulate != 0 also adds every key's softmax weights, summed over the query rows of its kv head, to cache->weights.
  * q, out: fp32 rows of head_dim at token * q_token + head * q_head + seq * q_seq floats (multiples of 4, 16-byte aligned);
- * out must not overlap q.  head_dim 32, 64, 96, 128 or 256, else UnsupportedOperation.
+ * out must not overlap q, nor its rows each other (stride 0 is refused; q, masks and an fp16 cache may have it).  head_dim 32, 64, 96, 128 or 256, else UnsupportedOperation.
  * `workspace` (16-byte aligned, kcb_cache_attention_workspace_bytes of the same arguments, possibly 0) is used in stream order:
  * calls that share one must not overlap. */
 typedef struct {

@@ -302,6 +302,7 @@ int kcb_ggml_flash_attn(void* h, const kcb_tensor* dst) {
     if (Hkv <= 0 || H % Hkv) return KCB_INVALID_VALUE;
     const float max_bias = param_f32(dst, 1), softcap = param_f32(dst, 2);
     if (max_bias != 0.0f || softcap != 0.0f) {  // capped or distance-biased scores: the KV-cache attention
+        if (q->ne[3] != 1 || (mask && (mask->ne[2] != 1 || mask->ne[3] != 1))) return KCB_UNSUPPORTED_OPERATION;  // one sequence, one mask
         auto& c = *static_cast<Ctx*>(h);
         kcb_kv_cache cache{};
         cache.bits = KCB_CACHE_F16, cache.n_seqs = 1, cache.kv_heads = Hkv, cache.head_dim = D, cache.capacity = T;

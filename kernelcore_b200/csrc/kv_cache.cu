@@ -417,6 +417,11 @@ int cache_ok(const kcb_kv_cache* c) {
     }
     return KCB_SUCCESS;
 }
+// Sequences, heads or slots that share their rows (stride 0) can be read, but two of them would write to the same place.
+bool rows_apart(const kcb_kv_cache* c) {
+    if (c->bits != KCB_CACHE_F16) return true;
+    return (c->n_seqs <= 1 || (c->k_seq && c->v_seq)) && (c->kv_heads <= 1 || (c->k_head && c->v_head)) && (c->capacity <= 1 || (c->k_row && c->v_row));
+}
 size_t moves_offset(const kcb_kv_cache* c) { return (static_cast<size_t>(c->n_seqs) * c->kv_heads * 4 + 15) / 16 * 16; }
 // CTAs of the rows-in and rows-out kernels for one sequence.
 unsigned row_blocks(const kcb_kv_cache* c, int tokens) {
@@ -484,8 +489,11 @@ AttnCut attn_cut(const kcb_kv_cache* c, const kcb_cache_attn* a) {
 int attn_ok(const kcb_kv_cache* c, const kcb_cache_attn* a) {
     if (const int e = cache_ok(c); e != KCB_SUCCESS) return e;
     if (!a || a->n_tokens < 0 || a->heads <= 0 || a->heads % c->kv_heads || !std::isfinite(a->scale) || !(a->softcap >= 0.0f) || !std::isfinite(a->softcap) ||
-        !(a->max_bias >= 0.0f) || !std::isfinite(a->max_bias))
+        !(a->max_bias >= 0.0f) || !std::isfinite(a->max_bias) || !std::isfinite(a->scale * kLog2e))
         return KCB_INVALID_VALUE;
+    // scores over their cap, and the cap, stay far inside fp32's range
+    if (const float bend = std::fabs(a->scale) / a->softcap; a->softcap > 0.0f && a->scale != 0.0f && !(bend >= 1e-20f && bend <= 1e20f)) return KCB_INVALID_VALUE;
+    if (!std::isfinite(a->softcap * kLog2e)) return KCB_INVALID_VALUE;
     const long long rows = static_cast<long long>(a->n_tokens) * (a->heads / c->kv_heads);
     if (rows > (1 << 24)) return KCB_INVALID_VALUE;
     if ((a->q_doc == nullptr) != (a->k_doc == nullptr)) return KCB_INVALID_VALUE;
@@ -519,7 +527,7 @@ size_t kcb_cache_bytes(int bits, int n_seqs, int kv_heads, int head_dim, int cap
 
 int kcb_cache_append(const kcb_kv_cache* c, const float* k, const float* v, int n_tokens, int64_t token_stride, int64_t seq_stride, void* stream) {
     if (const int e = cache_ok(c); e != KCB_SUCCESS) return e;
-    if (!c->n_keys || !k || !v || n_tokens < 0 || token_stride < 0 || seq_stride < 0) return KCB_INVALID_VALUE;
+    if (!c->n_keys || !k || !v || n_tokens < 0 || token_stride < 0 || seq_stride < 0 || !rows_apart(c)) return KCB_INVALID_VALUE;
     if (misaligned(k, 16) || misaligned(v, 16) || token_stride % 4 || seq_stride % 4) return KCB_INVALID_POINTER;
     if (static_cast<long long>(n_tokens) * c->kv_heads > kMaxRows) return KCB_INVALID_VALUE;
     if (n_tokens == 0 || c->n_seqs == 0) return KCB_SUCCESS;
@@ -559,7 +567,8 @@ size_t kcb_cache_evict_workspace_bytes(const kcb_kv_cache* c, int keep) {
 
 int kcb_cache_evict(const kcb_kv_cache* c, int keep, int recent, void* workspace, size_t workspace_bytes, void* stream) {
     if (const int e = cache_ok(c); e != KCB_SUCCESS) return e;
-    if (!c->n_keys || !c->next_pos || !c->positions || !c->weights || keep <= 0 || recent < 0 || recent > keep) return KCB_INVALID_VALUE;
+    if (!c->n_keys || !c->next_pos || !c->positions || !c->weights || keep <= 0 || recent < 0 || recent > keep || !rows_apart(c))
+        return KCB_INVALID_VALUE;
     if (keep >= c->capacity || c->n_seqs == 0) return KCB_SUCCESS;  // no sequence can hold more
     if (!workspace || workspace_bytes < kcb_cache_evict_workspace_bytes(c, keep)) return KCB_INVALID_VALUE;
     if (misaligned(workspace, 16)) return KCB_INVALID_POINTER;
@@ -592,6 +601,7 @@ int kcb_cache_attention(const kcb_kv_cache* c, const kcb_cache_attn* a, const fl
     if (!q || !out) return KCB_INVALID_VALUE;
     if (misaligned(q, 16) || misaligned(out, 16)) return KCB_INVALID_POINTER;
     if (a->n_tokens == 0 || c->n_seqs == 0) return KCB_SUCCESS;
+    if ((a->n_tokens > 1 && !a->out_token) || (a->heads > 1 && !a->out_head) || (c->n_seqs > 1 && !a->out_seq)) return KCB_INVALID_VALUE;  // rows on top of each other
     const AttnCut cut = attn_cut(c, a);
     const size_t need = cut.bytes();
     if (need && (!workspace || workspace_bytes < need)) return KCB_INVALID_VALUE;

@@ -50,6 +50,12 @@ def _launch(fn, device: torch.device, *args) -> None:
         lib.check(status, fn.__name__)
 
 
+def _used_here(t: torch.Tensor, home: int) -> None:
+    """A workspace of stream `home` that went to the current stream: its memory is not given away while that still runs."""
+    if _stream(t.device.index) != home:
+        t.record_stream(torch.cuda.current_stream(t.device))
+
+
 def _on(t: torch.Tensor, dtype, shape, what: str, device) -> int:
     if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.device != device:
         raise ValueError(f"{what}: a contiguous {dtype} tensor of shape {tuple(shape)} on {device} is needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
@@ -136,13 +142,15 @@ class KVCache:
         if ws is None:
             n = max(16, _L.kcb_cache_evict_workspace_bytes(self._ref, keep))
             buf = torch.empty(n, dtype=torch.uint8, device=self.device)
-            ws = self._evict_ws[keep] = (buf, buf.data_ptr(), n)
-        _launch(_L.kcb_cache_evict, self.device, self._ref, keep, recent, ws[1], ws[2])
+            ws = self._evict_ws[keep] = (buf, buf.data_ptr(), n, _stream(self.device.index))
+        if self.n_seqs:
+            _launch(_L.kcb_cache_evict, self.device, self._ref, keep, recent, ws[1], ws[2])
+            _used_here(ws[0], ws[3])
 
 
 class Attention:
     """Attention of n_tokens query tokens per sequence over a cache, with the masks given here; holds the workspace, so two
-    calls of one object must not run at the same time.  What the masks contain may change between calls."""
+    calls of one object must not run at the same time, and which a graph that captured a call goes on using.  What the masks contain may change between calls."""
 
     def __init__(self, cache: KVCache, *, n_tokens: int, heads: int, scale: float | None = None, softcap: float = 0.0, max_bias: float = 0.0, causal: bool = True,
                  prefix: torch.Tensor | None = None, q_pos: torch.Tensor | None = None, q_doc: torch.Tensor | None = None, k_doc: torch.Tensor | None = None,
@@ -165,6 +173,7 @@ class Attention:
         n = _L.kcb_cache_attention_workspace_bytes(cache._ref, self._ref)
         self.workspace = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
         self._ws = (self.workspace.data_ptr(), n) if n else (None, 0)
+        self._home = _stream(dev.index)
 
     def __call__(self, q: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         """q: fp32 [n_seqs][n_tokens][heads][head_dim] (contiguous channels, any other strides); out likewise, not overlapping q."""
@@ -184,4 +193,6 @@ class Attention:
         if self._empty:
             return out
         _launch(_L.kcb_cache_attention, dev, self.cache._ref, self._ref, q.data_ptr(), out.data_ptr(), *self._ws)
+        if self.workspace is not None:
+            _used_here(self.workspace, self._home)
         return out

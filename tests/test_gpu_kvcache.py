@@ -550,3 +550,37 @@ def test_python_side_refusals():
         kvcache.Attention(c, n_tokens=1, heads=2)(torch.zeros(1, 1, 2, 64))
     with pytest.raises(ValueError):
         kvcache.Attention(c, n_tokens=1, heads=2, mask=torch.zeros(1, 1, 9, dtype=torch.float16, device="cuda"))
+
+
+def test_objects_created_on_one_stream_and_dropped_after_use_on_another():
+    """The workspace of a dropped object is not handed to the next tensor while the call on the other stream still uses it."""
+    c, k, v, gen = filled(4, 1, 20000, 2, 64, [20000], seed=3)
+    q = torch.randn(1, 1, 8, 64, generator=gen, device="cuda")
+    want = kvcache.Attention(c, n_tokens=1, heads=8)(q)
+    out, side = torch.empty_like(want), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    a = kvcache.Attention(c, n_tokens=1, heads=8)
+    n = a.workspace.numel()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        a(q, out)
+    del a
+    for _ in range(4):
+        torch.empty(n, dtype=torch.uint8, device="cuda").fill_(0x7F)   # would be the workspace
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(out, want)
+
+
+def test_evict_on_another_stream_and_with_no_sequence():
+    c, k, v, gen = filled(16, 2, 300, 2, 64, [300, 200], seed=4, evictable=True)
+    c.weights.uniform_(0, 1, generator=gen)
+    d = kvcache.KVCache(c.k.clone(), c.v.clone(), kv_heads=2, head_dim=64, capacity=300, n_keys=c.n_keys.clone(), next_pos=c.next_pos.clone(),
+                        positions=c.positions.clone(), weights=c.weights.clone())
+    c.evict(100, 10)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        d.evict(100, 10)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(c.n_keys, d.n_keys) and torch.equal(c.positions[:, :, :100], d.positions[:, :, :100]) and torch.equal(c.k[:, :100], d.k[:, :100])
+    kvcache.KVCache.empty(0, 2, 64, 300, evictable=True).evict(100, 10)

@@ -112,3 +112,25 @@ def test_python_side_refuses_tensors_that_do_not_fit():
     cpu = torch.zeros(1, 4, 2, 64, dtype=torch.float16)
     with pytest.raises(ValueError):
         kvcache.KVCache(cpu, cpu, kv_heads=2, head_dim=64, capacity=4)
+
+
+@pytest.mark.parametrize("scale, softcap, fine", [(0.125, 1e30, False), (0.125, 1e19, True), (1e10, 1e-15, False), (0.125, 3e38, False), (3e38, 0.0, False), (0.0, 1e30, True),
+                                                 (0.125, 50.0, True), (-0.125, 1e10, True), (1e10, 0.0, True)])
+def test_caps_and_scales_stay_inside_the_range_of_fp32(scale, softcap, fine):
+    c, a = cache(capacity=5000, n_seqs=1), attn(scale=scale, softcap=softcap)
+    assert (L.kcb_cache_attention_workspace_bytes(C.byref(c), C.byref(a)) > 0) == fine
+    assert attention(c, a, ws=None, ws_bytes=0) == INVALID_VALUE   # refused for the cap, else for the missing workspace
+
+
+@pytest.mark.parametrize("kw", [dict(k_seq=0), dict(v_seq=0), dict(k_head=0), dict(v_row=0)])
+def test_shared_rows_are_read_only(kw):
+    c = cache(**kw)
+    assert L.kcb_cache_append(C.byref(c), GOOD, GOOD, 1, 256, 256, None) == INVALID_VALUE
+    assert L.kcb_cache_evict(C.byref(c), 10, 2, GOOD, 1 << 30, None) == INVALID_VALUE
+    assert attention(c, attn(n_tokens=0), ws=None, ws_bytes=0) == OK
+
+
+def test_outputs_on_top_of_each_other_are_refused():
+    c = cache(positions=None, capacity=5000)
+    for kw in (dict(n_tokens=2, out_token=0), dict(out_head=0), dict(out_seq=0)):
+        assert attention(c, attn(**kw)) == INVALID_VALUE
