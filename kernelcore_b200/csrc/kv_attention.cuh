@@ -952,63 +952,81 @@ struct QTile {
     static constexpr int kSums = kYsc + kRows * 4;                       // [row][NB + 1]: one word more than blocks against bank conflicts
     static constexpr int kBytes = (kSums + kRows * (D / 32 + 1) * 4 + 15) / 16 * 16;
 };
+// One row by eight lanes: piece i * 8 + l8 of 8 channels into x[i], then scaled and split into the tile.
+template <int D>
+struct QPieces {
+    static constexpr int kCh = D / 8, kPer = (kCh + 7) / 8;
+    float x[kPer][8];
+};
+template <int D>
+__device__ __forceinline__ void fetch_q_row(const AttnP& P, int s, int kvh, int row, int l8, QPieces<D>& q) {
+    constexpr int kCh = QPieces<D>::kCh;
+    const bool ok = row < P.rows;
+    const int token = (ok ? row : 0) / P.group, head = kvh * P.group + (ok ? row : 0) % P.group;
+    const float* qp = P.q + static_cast<size_t>(s) * P.q_seq + static_cast<size_t>(token) * P.q_token + static_cast<size_t>(head) * P.q_head;
+#pragma unroll
+    for (int i = 0; i < QPieces<D>::kPer; ++i) {
+        const int ch = i * 8 + l8;
+        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f), b = a;
+        if (ok && ch < kCh) a = reinterpret_cast<const float4*>(qp)[2 * ch], b = reinterpret_cast<const float4*>(qp)[2 * ch + 1];
+        q.x[i][0] = a.x, q.x[i][1] = a.y, q.x[i][2] = a.z, q.x[i][3] = a.w, q.x[i][4] = b.x, q.x[i][5] = b.y, q.x[i][6] = b.z, q.x[i][7] = b.w;
+    }
+}
+template <int D, int FMT>
+__device__ __forceinline__ void put_q_row(const AttnP& P, uint8_t* qt, int r, int l8, const QPieces<D>& q) {
+    using Q = QTile<D>;
+    constexpr int kCh = QPieces<D>::kCh, kPer = QPieces<D>::kPer;
+    const float(&x)[kPer][8] = q.x;
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(x[i][k]));
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    float up, down;
+    row_scale(amax, up, down);
+    if (l8 == 0) reinterpret_cast<float*>(qt + Q::kYsc)[r] = P.sc * down * kCodeUp<FMT>;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int ch = i * 8 + l8;
+        if (FMT == 16) {
+            if (ch < kCh) {
+                uint4 hi, lo;
+                split2(x[i][0] * up, x[i][1] * up, hi.x, lo.x);
+                split2(x[i][2] * up, x[i][3] * up, hi.y, lo.y);
+                split2(x[i][4] * up, x[i][5] * up, hi.z, lo.z);
+                split2(x[i][6] * up, x[i][7] * up, hi.w, lo.w);
+                *reinterpret_cast<uint4*>(qt + r * Q::kRow + ch * 16) = hi;
+                *reinterpret_cast<uint4*>(qt + Q::kLo + r * Q::kRow + ch * 16) = lo;
+            }
+        } else {
+            const int b = ch / 4, c = ch % 4;  // piece c of block b: its four pairs (k, k + 4) go to four k places
+            float sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                sum += x[i][k] + x[i][k + 4];
+                if (ch < kCh) {
+                    unsigned hi, lo;
+                    split2(x[i][k] * up, x[i][k + 4] * up, hi, lo);
+                    const int at = r * Q::kRow + 2 * (16 * (2 * b + (k >> 1)) + 8 * (k & 1) + 2 * c);
+                    *reinterpret_cast<unsigned*>(qt + at) = hi;
+                    *reinterpret_cast<unsigned*>(qt + Q::kLo + at) = lo;
+                }
+            }
+            sum = quad_sum(sum);
+            if (ch < kCh && c == 0) reinterpret_cast<float*>(qt + Q::kSums)[r * (D / 32 + 1) + b] = sum * up * (1.0f / kCodeUp<FMT>);
+        }
+    }
+}
 template <int D, int FMT>
 __device__ __forceinline__ void load_q_tile(const AttnP& P, int s, int kvh, int row0, uint8_t* qt, int tid) {
-    using Q = QTile<D>;
-    constexpr int kCh = D / 8, kPer = (kCh + 7) / 8;  // pieces of 8 channels, eight lanes to a row
     const int l8 = tid & 7;
 #pragma unroll 1
-    for (int r = tid >> 3; r < Q::kRows; r += 16) {
-        const int row = row0 + r;
-        const bool ok = row < P.rows;
-        const int token = (ok ? row : 0) / P.group, head = kvh * P.group + (ok ? row : 0) % P.group;
-        const float* qp = P.q + static_cast<size_t>(s) * P.q_seq + static_cast<size_t>(token) * P.q_token + static_cast<size_t>(head) * P.q_head;
-        float x[kPer][8], amax = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int ch = i * 8 + l8;
-            float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f), b = a;
-            if (ok && ch < kCh) a = reinterpret_cast<const float4*>(qp)[2 * ch], b = reinterpret_cast<const float4*>(qp)[2 * ch + 1];
-            x[i][0] = a.x, x[i][1] = a.y, x[i][2] = a.z, x[i][3] = a.w, x[i][4] = b.x, x[i][5] = b.y, x[i][6] = b.z, x[i][7] = b.w;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(x[i][k]));
-        }
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        float up, down;
-        row_scale(amax, up, down);
-        if (l8 == 0) reinterpret_cast<float*>(qt + Q::kYsc)[r] = P.sc * down * kCodeUp<FMT>;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int ch = i * 8 + l8;
-            if (FMT == 16) {
-                if (ch < kCh) {
-                    uint4 hi, lo;
-                    split2(x[i][0] * up, x[i][1] * up, hi.x, lo.x);
-                    split2(x[i][2] * up, x[i][3] * up, hi.y, lo.y);
-                    split2(x[i][4] * up, x[i][5] * up, hi.z, lo.z);
-                    split2(x[i][6] * up, x[i][7] * up, hi.w, lo.w);
-                    *reinterpret_cast<uint4*>(qt + r * Q::kRow + ch * 16) = hi;
-                    *reinterpret_cast<uint4*>(qt + Q::kLo + r * Q::kRow + ch * 16) = lo;
-                }
-            } else {
-                const int b = ch / 4, c = ch % 4;  // piece c of block b: its four pairs (k, k + 4) go to four k places
-                float sum = 0.0f;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    sum += x[i][k] + x[i][k + 4];
-                    if (ch < kCh) {
-                        unsigned hi, lo;
-                        split2(x[i][k] * up, x[i][k + 4] * up, hi, lo);
-                        const int at = r * Q::kRow + 2 * (16 * (2 * b + (k >> 1)) + 8 * (k & 1) + 2 * c);
-                        *reinterpret_cast<unsigned*>(qt + at) = hi;
-                        *reinterpret_cast<unsigned*>(qt + Q::kLo + at) = lo;
-                    }
-                }
-                sum = quad_sum(sum);
-                if (ch < kCh && c == 0) reinterpret_cast<float*>(qt + Q::kSums)[r * (D / 32 + 1) + b] = sum * up * (1.0f / kCodeUp<FMT>);
-            }
-        }
+    for (int r = tid >> 3; r < QTile<D>::kRows; r += 16) {
+        QPieces<D> q;
+        fetch_q_row<D>(P, s, kvh, row0 + r, l8, q);
+        put_q_row<D, FMT>(P, qt, r, l8, q);
     }
 }
 // Products of this warp's 16 rows (row r0 of the query tile on) with NTL n-tiles of 8 slots, from 16-slot block `blk0` of a key
@@ -1361,69 +1379,107 @@ __global__ void __launch_bounds__(128) attn_tile_kernel(const __grid_constant__ 
 
 // ---- attention weights per key ---------------------------------------------------------------------------------------------------
 // weights[t] += sum over the rows of a kv head of softmax(z)_t, from the rows' final maximum and sum.  A CTA owns 64 slots and
-// goes over all rows in order, so nothing is added atomically and the result does not depend on timing.
+// goes over all rows in order, so nothing is added atomically and the result does not depend on timing.  Sixteen warps: four blocks of
+// 16 slots times the four steps of 16 rows of a query tile, whose successor is on its way from memory meanwhile.
 template <int D, int FMT>
 struct WeightsCfg {
+    static constexpr int kThreads = 512;
     static constexpr int kOffK = QTile<D>::kBytes;
-    static constexpr int kSmem = kOffK + Tile<D, FMT>::bytes(64);
+    static constexpr int kOffRows = kOffK + Tile<D, FMT>::bytes(64);  // per row: RowInfo, {reference, 1 / sum}
+    static constexpr int kOffMl = kOffRows + QTile<D>::kRows * static_cast<int>(sizeof(RowInfo));
+    static constexpr int kOffSum = kOffMl + QTile<D>::kRows * 8;      // [step][slot]
+    static constexpr int kSmem = kOffSum + 4 * 64 * 4;
+    static_assert(kOffRows % 16 == 0 && kOffMl % 8 == 0 && kThreads == 8 * QTile<D>::kRows);
 };
-template <int D, int FMT>
-__global__ void __launch_bounds__(128) attn_weights_kernel(const __grid_constant__ AttnP P) {
+// GEN = false: neither cap nor bias, documents or mask.  The two branch-free tests that are left decide by the key's position alone.
+template <int D, int FMT, bool GEN>
+__global__ void __launch_bounds__(WeightsCfg<D, FMT>::kThreads, D <= 128 ? 2 : 1) attn_weights_kernel(const __grid_constant__ AttnP P) {
     using C = WeightsCfg<D, FMT>;
     using Q = QTile<D>;
     extern __shared__ __align__(16) uint8_t sm[];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
+    const int tid = threadIdx.x, lane = tid & 31, blk = (tid >> 5) & 3, step = tid >> 7, g = lane >> 2, c = lane & 3;
     const int t0 = blockIdx.x * 64, kvh = blockIdx.y, s = blockIdx.z;
     grid_dependency_wait();
     const int n = seq_keys(P, s);
     if (t0 >= n) return;
     const uint8_t* kt = sm + C::kOffK;
-    load_tile<D, FMT, 64, 128>(P, P.k, P.k_row, P.k_head, P.k_seq, s, kvh, t0, n, smem_u32(kt), tid);
+    if (tid < 128) load_tile<D, FMT, 64, 128>(P, P.k, P.k_row, P.k_head, P.k_seq, s, kvh, t0, n, smem_u32(kt), tid);
     cp_commit();
     const int prefix = P.prefix ? P.prefix[s] : 0;
     KeyInfo key[4];
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) key[j] = key_info(P, s, kvh, t0 + warp * 16 + slot_of<FMT>(c, j), n);
+    for (int j = 0; j < 4; ++j) {
+        key[j] = key_info(P, s, kvh, t0 + blk * 16 + slot_of<FMT>(c, j), n);
+        if (!GEN && (!P.causal || key[j].pos < prefix)) key[j].pos = INT32_MIN;  // every row sees it (what lies behind n is not stored)
+    }
     int row0 = 0;
     if (P.causal && !P.positions && !P.q_pos && t0 >= prefix) {  // rows in front of the first token that sees slot t0
         const int first = t0 - row_pos(P, s, n, 0);
-        if (first > 0) row0 = min(P.rows, first * P.group) / Q::kRows * Q::kRows;
+        if (first > 0) row0 = static_cast<int>(min(static_cast<long long>(P.rows), static_cast<long long>(first) * P.group)) / Q::kRows * Q::kRows;
     }
+    RowInfo* infos = reinterpret_cast<RowInfo*>(sm + C::kOffRows);
+    float2* mls = reinterpret_cast<float2*>(sm + C::kOffMl);
+    // a thread's part of a query tile: pieces of row tid / 8, and for one of the eight what that row needs to know
+    const int qr = tid >> 3, l8 = tid & 7;
+    QPieces<D> q;
+    RowInfo info{};
+    float2 ml{};
+    auto fetch = [&](int first) {
+        const int row = first + qr;
+        fetch_q_row<D>(P, s, kvh, row, l8, q);
+        if (l8 == 0) {
+            info = row_info(P, s, kvh, n, row);
+            ml = info.valid ? P.final_ml[(static_cast<size_t>(s) * P.kv_heads + kvh) * P.rows + row] : make_float2(0.0f, 0.0f);
+        }
+    };
+    if (row0 < P.rows) fetch(row0);
     for (; row0 < P.rows; row0 += Q::kRows) {
-        load_q_tile<D, FMT>(P, s, kvh, row0, sm, tid);
+        put_q_row<D, FMT>(P, sm, qr, l8, q);
+        if (l8 == 0) infos[qr] = info, mls[qr] = ml.y != 0.0f ? make_float2(ml.x - kPShift, 1.0f / ml.y) : make_float2(0.0f, 0.0f);
+        if (row0 + Q::kRows < P.rows) fetch(row0 + Q::kRows);
         cp_wait<0>();
         __syncthreads();
-#pragma unroll 1
-        for (int r0 = 0; r0 < Q::kRows && row0 + r0 < P.rows; r0 += 16) {
+        const int r0 = step * 16;
+        if (row0 + r0 < P.rows) {
             float sc[2][4];
-            scores16<D, FMT, 2, 64>(sc, sm, r0, kt, warp, lane);
+            scores16<D, FMT, 2, 64>(sc, sm, r0, kt, blk, lane);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int row = row0 + r0 + 8 * h + g;
-                const RowInfo ri = row_info(P, s, kvh, n, row);
-                const float2 ml = ri.valid ? P.final_ml[(static_cast<size_t>(s) * P.kv_heads + kvh) * P.rows + row] : make_float2(0.0f, 0.0f);
-                const float inv = ml.y != 0.0f ? 1.0f / ml.y : 0.0f, ref = ml.x - kPShift;
-                const float ys = reinterpret_cast<const float*>(sm + Q::kYsc)[r0 + 8 * h + g];
+                const int r = r0 + 8 * h + g;
+                const float2 m = mls[r];
+                const float ys = reinterpret_cast<const float*>(sm + Q::kYsc)[r];
+                if (!GEN) {
+                    const int pos = infos[r].pos;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float p = ex2(fmaf(sc[j >> 1][2 * h + (j & 1)], ys, -m.x)) * m.y;
+                        sum[j] += key[j].pos <= pos && m.y != 0.0f ? p : 0.0f;
+                    }
+                    continue;
+                }
+                const RowInfo ri = infos[r];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float y = general_score(P, sc[j >> 1][2 * h + (j & 1)] * ys, ri, key[j], t0 + warp * 16 + slot_of<FMT>(c, j), n, prefix);
-                    sum[j] += y == -INFINITY ? 0.0f : ex2(y - ref) * inv;
+                    const float y = general_score(P, sc[j >> 1][2 * h + (j & 1)] * ys, ri, key[j], t0 + blk * 16 + slot_of<FMT>(c, j), n, prefix);
+                    sum[j] += y == -INFINITY || m.y == 0.0f ? 0.0f : ex2(y - m.x) * m.y;
                 }
             }
         }
         __syncthreads();
     }
     cp_wait<0>();
+    float* sums = reinterpret_cast<float*>(sm + C::kOffSum);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         float v = sum[j];
         v += __shfl_xor_sync(0xffffffffu, v, 4);
         v += __shfl_xor_sync(0xffffffffu, v, 8);
         v += __shfl_xor_sync(0xffffffffu, v, 16);
-        const int t = t0 + warp * 16 + slot_of<FMT>(c, j);
-        if (g == 0 && t < n) P.weights[(static_cast<size_t>(s) * P.kv_heads + kvh) * P.cap + t] += v;
+        if (g == 0) sums[step * 64 + blk * 16 + slot_of<FMT>(c, j)] = v;
     }
+    __syncthreads();
+    if (tid < 64 && t0 + tid < n) P.weights[(static_cast<size_t>(s) * P.kv_heads + kvh) * P.cap + t0 + tid] += (sums[tid] + sums[64 + tid]) + (sums[128 + tid] + sums[192 + tid]);
 }
 
 // ---- launches --------------------------------------------------------------------------------------------------------------------
@@ -1483,9 +1539,11 @@ int attn_launch_kernels(const AttnP& P, bool general, AttnKernel which, cudaStre
         if (e != KCB_SUCCESS) return e;
     }
     if (P.final_ml) {
-        static PerDeviceFlag raised;
-        if (!raise_dynamic_smem(attn_weights_kernel<D, FMT>, WeightsCfg<D, FMT>::kSmem, raised)) return KCB_LAUNCH_FAILURE;
-        return launch_dependent(attn_weights_kernel<D, FMT>, dim3((P.cap + 63) / 64, P.kv_heads, P.n_seqs), 128, WeightsCfg<D, FMT>::kSmem, st, P);
+        static PerDeviceFlag raised[2];
+        const bool gen = P.cap_out != 0.0f || P.bias_step != 0.0f || P.q_doc || P.mask;
+        const auto kernel = gen ? attn_weights_kernel<D, FMT, true> : attn_weights_kernel<D, FMT, false>;
+        if (!raise_dynamic_smem(kernel, WeightsCfg<D, FMT>::kSmem, raised[gen])) return KCB_LAUNCH_FAILURE;
+        return launch_dependent(kernel, dim3((P.cap + 63) / 64, P.kv_heads, P.n_seqs), WeightsCfg<D, FMT>::kThreads, WeightsCfg<D, FMT>::kSmem, st, P);
     }
     return KCB_SUCCESS;
 }
