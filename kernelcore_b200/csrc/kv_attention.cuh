@@ -63,16 +63,23 @@ struct AttnP {
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_dependents_may_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 template <class... P, class... A>
-inline int launch_dependent(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
+inline int launch_clusters(void (*kernel)(P...), dim3 grid, int cluster, int threads, size_t smem, cudaStream_t st, A... args) {  // cluster: CTAs along x
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid, cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr, cfg.numAttrs = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster), attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr, cfg.numAttrs = cluster > 1 ? 2 : 1;
     if (cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess) return KCB_SUCCESS;
     cudaGetLastError();
     return KCB_LAUNCH_FAILURE;
+}
+
+template <class... P, class... A>
+inline int launch_dependent(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
+    return launch_clusters(kernel, grid, 1, threads, smem, st, args...);
 }
 
 // ---- small device helpers ------------------------------------------------------------------------------------------
@@ -1380,7 +1387,8 @@ __global__ void __launch_bounds__(128) attn_tile_kernel(const __grid_constant__ 
 // ---- attention weights per key ---------------------------------------------------------------------------------------------------
 // weights[t] += sum over the rows of a kv head of softmax(z)_t, from the rows' final maximum and sum.  A CTA owns 64 slots and
 // goes over all rows in order, so nothing is added atomically and the result does not depend on timing.  Sixteen warps: four blocks of
-// 16 slots times the four steps of 16 rows of a query tile, whose successor is on its way from memory meanwhile.
+// 16 slots times the four steps of 16 rows of a query tile, whose successor is on its way from memory meanwhile.  Where there are
+// few slots, the CTAs of a cluster take the query tiles in turn, and the first one adds up their sums in order.
 template <int D, int FMT>
 struct WeightsCfg {
     static constexpr int kThreads = 512;
@@ -1393,12 +1401,12 @@ struct WeightsCfg {
 };
 // GEN = false: neither cap nor bias, documents or mask.  The two branch-free tests that are left decide by the key's position alone.
 template <int D, int FMT, bool GEN>
-__global__ void __launch_bounds__(WeightsCfg<D, FMT>::kThreads, D <= 128 ? 2 : 1) attn_weights_kernel(const __grid_constant__ AttnP P) {
+__global__ void __launch_bounds__(WeightsCfg<D, FMT>::kThreads, D <= 128 ? 2 : 1) attn_weights_kernel(const __grid_constant__ AttnP P, int ranks) {
     using C = WeightsCfg<D, FMT>;
     using Q = QTile<D>;
     extern __shared__ __align__(16) uint8_t sm[];
     const int tid = threadIdx.x, lane = tid & 31, blk = (tid >> 5) & 3, step = tid >> 7, g = lane >> 2, c = lane & 3;
-    const int t0 = blockIdx.x * 64, kvh = blockIdx.y, s = blockIdx.z;
+    const int t0 = blockIdx.x / ranks * 64, rank = blockIdx.x % ranks, kvh = blockIdx.y, s = blockIdx.z;
     grid_dependency_wait();
     const int n = seq_keys(P, s);
     if (t0 >= n) return;
@@ -1418,6 +1426,8 @@ __global__ void __launch_bounds__(WeightsCfg<D, FMT>::kThreads, D <= 128 ? 2 : 1
         const int first = t0 - row_pos(P, s, n, 0);
         if (first > 0) row0 = static_cast<int>(min(static_cast<long long>(P.rows), static_cast<long long>(first) * P.group)) / Q::kRows * Q::kRows;
     }
+    row0 += rank * Q::kRows;
+    const int stride = ranks * Q::kRows;
     RowInfo* infos = reinterpret_cast<RowInfo*>(sm + C::kOffRows);
     float2* mls = reinterpret_cast<float2*>(sm + C::kOffMl);
     // a thread's part of a query tile: pieces of row tid / 8, and for one of the eight what that row needs to know
@@ -1434,10 +1444,10 @@ __global__ void __launch_bounds__(WeightsCfg<D, FMT>::kThreads, D <= 128 ? 2 : 1
         }
     };
     if (row0 < P.rows) fetch(row0);
-    for (; row0 < P.rows; row0 += Q::kRows) {
+    for (; row0 < P.rows; row0 += stride) {
         put_q_row<D, FMT>(P, sm, qr, l8, q);
         if (l8 == 0) infos[qr] = info, mls[qr] = ml.y != 0.0f ? make_float2(ml.x - kPShift, 1.0f / ml.y) : make_float2(0.0f, 0.0f);
-        if (row0 + Q::kRows < P.rows) fetch(row0 + Q::kRows);
+        if (P.rows - row0 > stride) fetch(row0 + stride);
         cp_wait<0>();
         __syncthreads();
         const int r0 = step * 16;
@@ -1479,7 +1489,20 @@ __global__ void __launch_bounds__(WeightsCfg<D, FMT>::kThreads, D <= 128 ? 2 : 1
         if (g == 0) sums[step * 64 + blk * 16 + slot_of<FMT>(c, j)] = v;
     }
     __syncthreads();
-    if (tid < 64 && t0 + tid < n) P.weights[(static_cast<size_t>(s) * P.kv_heads + kvh) * P.cap + t0 + tid] += (sums[tid] + sums[64 + tid]) + (sums[128 + tid] + sums[192 + tid]);
+    float all = 0.0f;
+    if (tid < 64) all = (sums[tid] + sums[64 + tid]) + (sums[128 + tid] + sums[192 + tid]);
+    if (ranks > 1) {
+        if (tid < 64) sums[tid] = all;  // (only this thread read that word)
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (rank == 0 && tid < 64)
+            for (int i = 1; i < ranks; ++i) {
+                float x;
+                asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}" : "=f"(x) : "r"(smem_u32(sums + tid)), "r"(i) : "memory");
+                all += x;
+            }
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");  // their memory is read
+    }
+    if (rank == 0 && tid < 64 && t0 + tid < n) P.weights[(static_cast<size_t>(s) * P.kv_heads + kvh) * P.cap + t0 + tid] += all;
 }
 
 // ---- launches --------------------------------------------------------------------------------------------------------------------
@@ -1543,7 +1566,10 @@ int attn_launch_kernels(const AttnP& P, bool general, AttnKernel which, cudaStre
         const bool gen = P.cap_out != 0.0f || P.bias_step != 0.0f || P.q_doc || P.mask;
         const auto kernel = gen ? attn_weights_kernel<D, FMT, true> : attn_weights_kernel<D, FMT, false>;
         if (!raise_dynamic_smem(kernel, WeightsCfg<D, FMT>::kSmem, raised[gen])) return KCB_LAUNCH_FAILURE;
-        return launch_dependent(kernel, dim3((P.cap + 63) / 64, P.kv_heads, P.n_seqs), WeightsCfg<D, FMT>::kThreads, WeightsCfg<D, FMT>::kSmem, st, P);
+        const long long blocks = (P.cap + 63) / 64, tiles = (P.rows + QTile<D>::kRows - 1) / QTile<D>::kRows;
+        int ranks = 1;  // clusters of up to 8 while the GPU has room for twice the CTAs
+        while (ranks < 8 && 2 * ranks <= tiles && 2 * ranks * blocks * P.kv_heads * P.n_seqs <= 2 * kSmCount) ranks *= 2;
+        return launch_clusters(kernel, dim3(static_cast<unsigned>(blocks) * ranks, P.kv_heads, P.n_seqs), ranks, WeightsCfg<D, FMT>::kThreads, WeightsCfg<D, FMT>::kSmem, st, P, ranks);
     }
     return KCB_SUCCESS;
 }

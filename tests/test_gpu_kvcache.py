@@ -584,3 +584,21 @@ def test_evict_on_another_stream_and_with_no_sequence():
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(c.n_keys, d.n_keys) and torch.equal(c.positions[:, :, :100], d.positions[:, :, :100]) and torch.equal(c.k[:, :100], d.k[:, :100])
     kvcache.KVCache.empty(0, 2, 64, 300, evictable=True).evict(100, 10)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("N, H, Hkv, D, cap, n", [(64, 4, 2, 64, 64, 64), (65, 2, 1, 128, 100, 100), (200, 2, 1, 128, 300, 290), (300, 8, 2, 64, 500, 400), (500, 2, 1, 32, 70, 70),
+                                                  (700, 1, 1, 256, 700, 700), (40, 4, 4, 96, 1300, 65)])
+def test_weights_of_prompts_by_one_cta_and_by_clusters(bits, N, H, Hkv, D, cap, n):
+    """Query tiles of 64 rows shared out over 1, 2, 4 or 8 CTAs, tiles that do not divide evenly, ranks that have none left."""
+    c, k, v, gen = filled(bits, 1, cap, Hkv, D, [n], seed=N + D, evictable=True)
+    q = torch.randn(1, N, H, D, generator=gen, device="cuda")
+    check(c, k, v, q, N, H, accumulate=True)
+    check(c, k, v, q, N, H, accumulate=True, softcap=10.0, prefix=torch.tensor([n // 2], dtype=torch.int32, device="cuda"))
+    w0 = c.weights.clone()
+    att = kvcache.Attention(c, n_tokens=N, heads=H, accumulate=True)
+    att(q)
+    first = c.weights.clone()
+    c.weights.copy_(w0)
+    att(q)
+    assert torch.equal(c.weights, first)   # the order of the sums is fixed
