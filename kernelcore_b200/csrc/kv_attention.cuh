@@ -454,6 +454,8 @@ constexpr float kCodeUp = FMT == 16 ? 1.0f : 1024.0f;
 // copies in flight, its own running maximum), so nothing waits for a neighbour; the eight rows' hi and lo halves are stacked
 // into one 16-row fragment, which makes the second half of the precision free of extra products.  16 slots a block for fp16 (whose
 // ring then fills the shared memory with eight warps), 32 for 4 bits.
+// Measured: 32 sequences of 4096 slots, 32 heads over 8, D = 128: fp16 110 us back to back = 4.9 TB/s (0.31 instructions issued per
+// cycle and scheduler: the latency of the ring), 4 bits 67 us = 2.5 TB/s (0.55 on 131072 slots: unpacking).
 // MODE 0: scores as they are; 1: with a cap or a distance bias, slot = position; 2: positions, documents or an additive mask too.
 // In the first two a row sees the slots below a limit.
 constexpr int kRowsWarps = 4;
@@ -1097,9 +1099,10 @@ __device__ __forceinline__ void scores16(float (&sc)[NTL][4], const uint8_t* qt,
 }
 
 // ---- tile kernel: 64 rows per CTA ---------------------------------------------------------------------------------------------
-// For prompts.  Four warps of 16 rows share every key and value tile; what bounds it is the tensor pipe (two products for
+// For prompts of the shapes that the tcgen05 kernel does not take.  Four warps of 16 rows share every key and value tile; what bounds it is the tensor pipe (two products for
 // each of the two contractions).  A tile's value products start from zero and are added to the running output in fp32, so
 // the length of the context never meets the rounding of the tensor cores' accumulation.
+// Measured: 2048 tokens over 2048 slots, 16 heads over 8, D = 256, no mask: 722 us = 95 TFLOP/s (fp16), 832 us (4 bits).
 template <int D, int FMT>
 struct TileCfg {
     static constexpr int kKeys = D >= 256 ? 32 : 64;
@@ -1389,6 +1392,9 @@ __global__ void __launch_bounds__(128) attn_tile_kernel(const __grid_constant__ 
 // goes over all rows in order, so nothing is added atomically and the result does not depend on timing.  Sixteen warps: four blocks of
 // 16 slots times the four steps of 16 rows of a query tile, whose successor is on its way from memory meanwhile.  Where there are
 // few slots, the CTAs of a cluster take the query tiles in turn, and the first one adds up their sums in order.
+// Bounded by issue slots: per 8 scores of a lane 32 products, their 24 fragment loads and some 60 instructions to sum weights.
+// Measured: 2048 tokens, 32 heads over 8, D = 128: 500 us (fp16), 750 (4 bits) behind 219 and 381 of attention; 300 tokens, 8 heads over
+// 2, over 500 slots 17 us in clusters of 8, 53 without.
 template <int D, int FMT>
 struct WeightsCfg {
     static constexpr int kThreads = 512;

@@ -18,6 +18,9 @@
 // a tensor copy brings along.  Looking for such values costs a third of the kernel's time, so the first pass does not: where an output
 // is not finite at its end, the CTA takes a second pass that does, clears them from the tiles, and gives them to the rows that see
 // them one by one.  (4-bit rows need none: the unpacking turns scales that are not finite into zeros.)
+// Bounded by the issue slots of the softmax warpgroups and, at two products for one, by the tensor pipe.  4096 tokens, 32 heads over 8,
+// D = 128: fp16 causal 270 us, all slots 450 us = 610 TFLOP/s (twice that in products), with a cap 416; 4 bits causal 520 us (unpacking
+// and three products for one).
 // Every wait is bounded: on expiry the CTA raises a flag that all roles poll, runs on without products, waits for its copies and
 // products in flight, counts the event, frees its TMEM and returns.
 #pragma once
