@@ -474,7 +474,8 @@ AttnCut attn_cut(const kcb_kv_cache* c, const kcb_cache_attn* a) {
     const long long want = (r.which == AttnKernel::tc ? 1 : 2) * kSmCount, least = 128;
     r.nsplit = static_cast<int>(std::max<long long>(1, std::min<long long>(want / std::max<long long>(ctas, 1), (c->capacity + least - 1) / least)));
     // A rows launch adds values up on the tensor cores, whose sums truncate: at most 2048 slots per split are 32 additions per warp
-    // (131072 4-bit rows, relative error against 64 bits: 6.4e-6 with 3543 slots a split, 2.8e-6 with 1771).  More splits than the
+    // (131072 4-bit rows, relative error against 64 bits: 6.4e-6 with 3543 slots a split, 2.7e-6 with 1771, 1.3e-6 with 885, which take
+    // 70 us instead of 62).  More splits than the
     // GPU holds CTAs of (two per SM) come in whole rounds of them: 131072 rows of 8 heads 62 us in 74 splits, 67 us in 64.
     if (r.which == AttnKernel::rows && ctas) {
         const long long need = std::max<long long>(r.nsplit, (c->capacity + 2047) / 2048), round = 2 * kSmCount;
